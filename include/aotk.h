@@ -371,6 +371,52 @@ AOTK_API int aotk_watchdog_status(int device, uint32_t* status, int clear);
  * without faulting or hanging the GPU.  No reference counterpart. */
 AOTK_API int aotk_watchdog_selftest(void* stream);
 
+/* ---- microscaled 4-bit floating point (MX: e2m1 elements, blocks of 32) ---- */
+
+/* Layout of a quantised [rows, cols] matrix, cols a multiple of 32:
+ *   codes  [rows, cols / 2] bytes, the even column in the low nibble, e2m1
+ *          (sign, 2 exponent bits of bias 1, 1 mantissa bit);
+ *   scales [ceil(rows / 128)][ceil(cols / 128)][512] bytes: block j (columns
+ *          [32 j, 32 j + 32)) of row r has byte
+ *          (r % 32) * 16 + (r % 128 / 32) * 4 + j % 4 of tile
+ *          [r / 128][j / 4]; it stands for 2^(byte - 127), 255 for NaN.
+ *          Bytes of a tile that belong to no row or block are 0.
+ * Both 16-byte aligned. */
+
+/* Quantises x [rows, cols] (row stride x_stride elements; fp32, fp16 or bf16)
+ * along its rows: scale 2^(floor(log2 max|x|) - 2) per block (clamped to the
+ * byte's range), elements rounded to nearest even, magnitudes above 6 scales
+ * to 6.  A block with a NaN or an infinity reads back as NaN throughout.
+ * Writes every byte of both outputs.  No reference counterpart: the reference
+ * takes 8-bit operands that its caller has quantised
+ * (jit_kernel/gemm.py:199-248). */
+AOTK_API int aotk_mxfp4_quantize(void* codes, void* scales, const void* x, int64_t x_stride,
+                                 int64_t rows, int64_t cols, int dtype, void* stream);
+
+/* out[r, c] = element * scale, rounded once to dtype; out is dense. */
+AOTK_API int aotk_mxfp4_dequantize(void* out, const void* codes, const void* scales, int64_t rows,
+                                   int64_t cols, int dtype, void* stream);
+
+/* C[M, N] = A B^T over the values of A [M, K] and B [N, K] (both quantised
+ * along K), fp32 accumulation, one rounding to out_dtype (fp32, fp16, bf16). */
+AOTK_API int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, const void* b,
+                             const void* b_scales, int64_t M, int64_t N, int64_t K, int out_dtype,
+                             void* stream);
+
+/* The norms before and after a residual block, with its gate and residual
+ * scale, in one pass (all [rows, cols], one dtype, fp32 math):
+ *   h_out = residual_scale * residual + gate * rms(x) * post_weight
+ *   out   = rms(h) * pre_weight, rms(v) = v * rsqrt(mean(v^2) + eps)
+ * out is computed from the unrounded h.  gate (may be null) is [gate_rows,
+ * gate_cols]: gate_cols is cols or 1, gate_rows divides rows, and row r uses
+ * gate row r / (rows / gate_rows).  No reference counterpart: the reference
+ * composes its rmsnorm (aot_kernel/norm.py:9-18) with torch. */
+AOTK_API int aotk_sandwich_rmsnorm(void* out, void* h_out, const void* x, const void* residual,
+                                   const void* post_weight, const void* pre_weight,
+                                   const void* gate, int64_t gate_rows, int64_t gate_cols,
+                                   double residual_scale, int64_t rows, int64_t cols, double eps,
+                                   int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

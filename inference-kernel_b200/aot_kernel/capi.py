@@ -63,6 +63,11 @@ SIGNATURES: dict[str, list] = {
                             ctypes.c_size_t, _ptr],
     "aotk_scaled_gemm_simt": [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _int, _int,
                               _ptr],
+    "aotk_mxfp4_quantize": [_ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr],
+    "aotk_mxfp4_dequantize": [_ptr, _ptr, _ptr, _i64, _i64, _int, _ptr],
+    "aotk_mxfp4_gemm": [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr],
+    "aotk_sandwich_rmsnorm": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64,
+                              ctypes.c_double, _i64, _i64, ctypes.c_double, _int, _ptr],
 }
 
 
@@ -297,6 +302,28 @@ def scaled_gemm_simt(c, a, b, scale_a, scale_b, M, N, K, in_dtype, out_dtype, sc
                      stream=None) -> None:
     _call("aotk_scaled_gemm_simt", _p(c), _p(a), _p(b), _p(scale_a), _p(scale_b), M, N, K,
           in_dtype, out_dtype, scale_mode, _stream(stream))
+
+
+def mxfp4_quantize(codes, scales, x, x_stride, rows, cols, dtype, stream=None) -> None:
+    _call("aotk_mxfp4_quantize", _p(codes), _p(scales), _p(x), x_stride, rows, cols, dtype,
+          _stream(stream))
+
+
+def mxfp4_dequantize(out, codes, scales, rows, cols, dtype, stream=None) -> None:
+    _call("aotk_mxfp4_dequantize", _p(out), _p(codes), _p(scales), rows, cols, dtype,
+          _stream(stream))
+
+
+def mxfp4_gemm(c, a, a_scales, b, b_scales, M, N, K, out_dtype, stream=None) -> None:
+    _call("aotk_mxfp4_gemm", _p(c), _p(a), _p(a_scales), _p(b), _p(b_scales), M, N, K, out_dtype,
+          _stream(stream))
+
+
+def sandwich_rmsnorm(out, h_out, x, residual, post_weight, pre_weight, gate, gate_rows, gate_cols,
+                     residual_scale, rows, cols, eps, dtype, stream=None) -> None:
+    _call("aotk_sandwich_rmsnorm", _p(out), _p(h_out), _p(x), _p(residual), _p(post_weight),
+          _p(pre_weight), _p(gate), gate_rows, gate_cols, residual_scale, rows, cols, eps, dtype,
+          _stream(stream))
 
 
 def gemm_allreduce_tiles(M: int, N: int) -> int:

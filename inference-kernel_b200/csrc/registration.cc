@@ -1,7 +1,8 @@
 // torch operator library `aot_kernel`: the same schemas as the reference's
 // registration (aot_kernel/csrc/registration.cc:10-25) plus the fused ops
-// (silu_mul_forward, add_rmsnorm_forward, gemm_silu_mul) and scaled_gemm, the
-// 8-bit GEMM the reference provides as a Triton kernel.
+// (silu_mul_forward, add_rmsnorm_forward, gemm_silu_mul, sandwich_rmsnorm), scaled_gemm, the
+// 8-bit GEMM the reference provides as a Triton kernel, and the microscaled
+// 4-bit ops (mxfp4_quantize, mxfp4_dequantize, mxfp4_gemm).
 // Each kernel checks its tensors, pins the device, and calls the C ABI of
 // libaotk (include/aotk.h) on the current torch stream.  Unlike the
 // reference, launches go to at::cuda::getCurrentCUDAStream() under a device
@@ -12,6 +13,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
+
+#include <optional>
 
 #include "aotk.h"
 
@@ -334,6 +337,114 @@ void scaled_gemm(at::Tensor out, at::Tensor a, at::Tensor b, at::Tensor scale_a,
                op);
 }
 
+// Codes [rows, cols / 2] and scale tiles of a quantised matrix; returns cols.
+int64_t check_mxfp4(const at::Tensor& codes, const at::Tensor& scales, const char* op,
+                    const char* name) {
+  check_cuda(codes, op, name);
+  check_cuda(scales, op, "scales");
+  TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, "[", op, "] ",
+              name, " and its scales must be uint8");
+  TORCH_CHECK(codes.device() == scales.device(), "[", op, "] ", name,
+              " and its scales are not on the same device");
+  TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous(), "[", op, "] ", name,
+              " and its scales must be contiguous");
+  TORCH_CHECK(codes.dim() == 2 && codes.size(1) % 16 == 0, "[", op, "] ", name,
+              " must be [rows, cols / 2] with cols a multiple of 32, got ", codes.sizes());
+  const int64_t rows = codes.size(0), cols = 2 * codes.size(1);
+  TORCH_CHECK(scales.dim() == 3 && scales.size(0) == (rows + 127) / 128 &&
+                  scales.size(1) == (cols + 127) / 128 && scales.size(2) == 512,
+              "[", op, "] scales of ", name, " must be [", (rows + 127) / 128, ", ",
+              (cols + 127) / 128, ", 512], got ", scales.sizes());
+  return cols;
+}
+
+void mxfp4_quantize(at::Tensor codes, at::Tensor scales, at::Tensor x) {
+  const char* op = "mxfp4_quantize";
+  check_cuda(x, op, "x");
+  const int64_t cols = check_mxfp4(codes, scales, op, "codes");
+  TORCH_CHECK(codes.device() == x.device(), "[", op, "] x and codes are not on the same device");
+  TORCH_CHECK(x.dim() == 2 && x.size(0) == codes.size(0) && x.size(1) == cols, "[", op,
+              "] x must be [", codes.size(0), ", ", cols, "], got ", x.sizes());
+  const int64_t stride = row_stride(x, op, "x");
+  c10::cuda::CUDAGuard guard(x.device());
+  check_status(aotk_mxfp4_quantize(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), stride,
+                                   x.size(0), cols, aotk_dtype(x, op), current_stream(x)),
+               op);
+}
+
+void mxfp4_dequantize(at::Tensor out, at::Tensor codes, at::Tensor scales) {
+  const char* op = "mxfp4_dequantize";
+  check_cuda(out, op, "out");
+  const int64_t cols = check_mxfp4(codes, scales, op, "codes");
+  TORCH_CHECK(out.device() == codes.device(), "[", op, "] out and codes are not on the same device");
+  TORCH_CHECK(out.is_contiguous() && out.dim() == 2 && out.size(0) == codes.size(0) &&
+                  out.size(1) == cols,
+              "[", op, "] out must be a contiguous [", codes.size(0), ", ", cols, "], got ",
+              out.sizes());
+  c10::cuda::CUDAGuard guard(out.device());
+  check_status(aotk_mxfp4_dequantize(out.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                                     out.size(0), cols, aotk_dtype(out, op), current_stream(out)),
+               op);
+}
+
+void mxfp4_gemm(at::Tensor out, at::Tensor a, at::Tensor a_scales, at::Tensor b,
+                at::Tensor b_scales) {
+  const char* op = "mxfp4_gemm";
+  check_cuda(out, op, "out");
+  const int64_t K = check_mxfp4(a, a_scales, op, "a");
+  TORCH_CHECK(check_mxfp4(b, b_scales, op, "b") == K, "[", op, "] inner dims mismatch: ", K,
+              " vs ", 2 * b.size(1));
+  TORCH_CHECK(out.device() == a.device() && b.device() == a.device(), "[", op,
+              "] tensors are not on one device");
+  TORCH_CHECK(out.is_contiguous() && out.dim() == 2 && out.size(0) == a.size(0) &&
+                  out.size(1) == b.size(0),
+              "[", op, "] out must be a contiguous [", a.size(0), ", ", b.size(0), "], got ",
+              out.sizes());
+  c10::cuda::CUDAGuard guard(a.device());
+  check_status(aotk_mxfp4_gemm(out.data_ptr(), a.data_ptr(), a_scales.data_ptr(), b.data_ptr(),
+                               b_scales.data_ptr(), a.size(0), b.size(0), K, aotk_dtype(out, op),
+                               current_stream(a)),
+               op);
+}
+
+// gate: [gate_rows, cols] or [gate_rows, 1], row r of x using gate row
+// r / (rows / gate_rows).
+void sandwich_rmsnorm(at::Tensor out, at::Tensor h_out, at::Tensor x, at::Tensor residual,
+                      at::Tensor post_weight, at::Tensor pre_weight,
+                      std::optional<at::Tensor> gate, double residual_scale, double eps) {
+  const char* op = "sandwich_rmsnorm";
+  check_cuda(x, op, "x");
+  check_same(x, residual, op, "x", "residual");
+  check_same(x, post_weight, op, "x", "post_weight");
+  check_same(x, pre_weight, op, "x", "pre_weight");
+  TORCH_CHECK(x.dim() >= 1 && x.sizes() == residual.sizes(), "[", op,
+              "] x and residual shapes differ: ", x.sizes(), " vs ", residual.sizes());
+  TORCH_CHECK(x.is_contiguous() && residual.is_contiguous() && post_weight.is_contiguous() &&
+                  pre_weight.is_contiguous(),
+              "[", op, "] inputs must be contiguous");
+  const int64_t cols = x.size(-1);
+  TORCH_CHECK(post_weight.dim() == 1 && pre_weight.dim() == 1 && post_weight.size(0) == cols &&
+                  pre_weight.size(0) == cols,
+              "[", op, "] weights must be [x.size(-1)]");
+  check_out_like(out, x, op);
+  check_out_like(h_out, x, op);
+  if (x.numel() == 0) return;
+  const int64_t rows = x.numel() / cols;
+  if (gate) {
+    check_same(x, *gate, op, "x", "gate");
+    TORCH_CHECK(gate->is_contiguous() && gate->dim() == 2, "[", op,
+                "] gate must be a contiguous [gate_rows, cols] or [gate_rows, 1]");
+  }
+  c10::cuda::CUDAGuard guard(x.device());
+  check_status(aotk_sandwich_rmsnorm(out.data_ptr(), h_out.data_ptr(), x.data_ptr(),
+                                     residual.data_ptr(), post_weight.data_ptr(),
+                                     pre_weight.data_ptr(), gate ? gate->data_ptr() : nullptr,
+                                     gate ? gate->size(0) : 0, gate ? gate->size(1) : 0,
+                                     residual_scale, rows, cols, eps, aotk_dtype(x, op),
+                                     current_stream(x)),
+               op);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(aot_kernel, m) {
@@ -373,6 +484,21 @@ TORCH_LIBRARY(aot_kernel, m) {
       "scaled_gemm(Tensor! out, Tensor a, Tensor b, Tensor scale_a, Tensor scale_b, bool "
       "optimized) -> ()");
   m.impl("scaled_gemm", c10::kCUDA, &scaled_gemm);
+
+  m.def("mxfp4_quantize(Tensor! codes, Tensor! scales, Tensor x) -> ()");
+  m.impl("mxfp4_quantize", c10::kCUDA, &mxfp4_quantize);
+
+  m.def("mxfp4_dequantize(Tensor! out, Tensor codes, Tensor scales) -> ()");
+  m.impl("mxfp4_dequantize", c10::kCUDA, &mxfp4_dequantize);
+
+  m.def(
+      "mxfp4_gemm(Tensor! out, Tensor a, Tensor a_scales, Tensor b, Tensor b_scales) -> ()");
+  m.impl("mxfp4_gemm", c10::kCUDA, &mxfp4_gemm);
+
+  m.def(
+      "sandwich_rmsnorm(Tensor! out, Tensor! h_out, Tensor x, Tensor residual, Tensor post_weight, "
+      "Tensor pre_weight, Tensor? gate, float residual_scale, float eps) -> ()");
+  m.impl("sandwich_rmsnorm", c10::kCUDA, &sandwich_rmsnorm);
 }
 
 // `import aot_kernel._C` runs the static registration above; the module itself is empty.

@@ -282,3 +282,63 @@ def scaled_gemm_dequant_first(a_q, b_q, scale_a, scale_b, qdtype: str, out_dtype
     a = dequant(a_q, qdtype).astype(np.float32) * np.asarray(scale_a, np.float32).reshape(-1, 1)
     b = dequant(b_q, qdtype).astype(np.float32) * np.asarray(scale_b, np.float32).reshape(1, -1)
     return round_to((a.astype(np.float64) @ b.astype(np.float64)).astype(np.float32), out_dtype)
+
+
+# ---- microscaled 4-bit floating point (no reference counterpart) --------------
+
+E2M1 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def mxfp4_quantize(x: np.ndarray):
+    """(codes [rows, cols] of 0..15, scale bytes [rows, cols / 32]) of float32 x, in
+    64 bits: scale 2^clamp(floor(log2 max|x|) - 2, -127, 127); the nearest element,
+    ties to the even code; a block with a NaN or an infinity has byte 255 and codes 0."""
+    rows, cols = x.shape
+    b = np.asarray(x, dtype=np.float64).reshape(rows, cols // 32, 32)
+    bad = ~np.isfinite(b).all(-1)
+    b = np.where(bad[..., None], 0.0, b)
+    _, e = np.frexp(np.abs(b).max(-1))  # max = m * 2^e with m in [.5, 1)
+    exp = np.where(np.abs(b).max(-1) == 0, -127, np.maximum(e - 3, -127))
+    v = np.abs(b) / np.ldexp(1.0, exp)[..., None]
+    # the candidate pair around v: the lower neighbour and the distance past it
+    lo = np.clip(np.searchsorted(E2M1, v, side="right") - 1, 0, 6)
+    mid = (E2M1[lo] + E2M1[lo + 1]) / 2
+    code = lo + ((v > mid) | ((v == mid) & (lo % 2 == 1)))
+    code = code + 8 * np.signbit(b)
+    code = np.where(bad[..., None], 0, code)
+    return (code.reshape(rows, cols).astype(np.uint8),
+            np.where(bad, 255, exp + 127).astype(np.uint8))
+
+
+def mxfp4_pack(code: np.ndarray) -> np.ndarray:
+    """Codes [rows, cols] -> bytes [rows, cols / 2], the even column in the low nibble."""
+    return (code[:, 0::2] | (code[:, 1::2] << 4)).astype(np.uint8)
+
+
+def mxfp4_tile(scale: np.ndarray) -> np.ndarray:
+    """Scale bytes [rows, blocks] -> [ceil(rows/128), ceil(blocks/4), 512], byte by byte."""
+    rows, blocks = scale.shape
+    out = np.zeros(((rows + 127) // 128, (blocks + 3) // 4, 512), dtype=np.uint8)
+    for r in range(rows):
+        for j in range(blocks):
+            out[r // 128, j // 4, (r % 32) * 16 + (r % 128) // 32 * 4 + j % 4] = scale[r, j]
+    return out
+
+
+def mxfp4_values(code: np.ndarray, scale: np.ndarray) -> np.ndarray:
+    """The float64 values that codes [rows, cols] and scale bytes [rows, cols / 32] hold."""
+    v = E2M1[code & 7] * np.where(code & 8, -1.0, 1.0)
+    s = np.where(scale == 255, np.nan, np.ldexp(1.0, scale.astype(np.int64) - 127))
+    return v * np.repeat(s, 32, axis=1)
+
+
+def sandwich_rmsnorm(x, residual, post, pre, eps: float, gate=None, alpha: float = 1.0):
+    """(out, h, branch) in float64: branch = gate * rms(x) * post, h = alpha * residual +
+    branch, out = rms(h) * pre, none of them rounded."""
+    x, residual = np.asarray(x, np.float64), np.asarray(residual, np.float64)
+    branch = x / np.sqrt(np.mean(x * x, -1, keepdims=True) + eps) * np.asarray(post, np.float64)
+    if gate is not None:
+        branch = branch * np.asarray(gate, np.float64)
+    h = alpha * residual + branch
+    out = h / np.sqrt(np.mean(h * h, -1, keepdims=True) + eps) * np.asarray(pre, np.float64)
+    return out, h, branch
