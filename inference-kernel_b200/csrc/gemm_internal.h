@@ -82,6 +82,7 @@ int watchdog_selftest(void* stream);
 
 // Watchdog words of the tensor-core kernels (OR-ed into *status).
 int tc_watchdog(uint32_t* status, bool clear);
+int mxfp4_watchdog(uint32_t* status, bool clear);
 int skinny_watchdog(uint32_t* status, bool clear);
 
 // Raises the dynamic shared-memory limit of `kernel` to `bytes` once per device.

@@ -2,100 +2,428 @@
 // A [M, K / 2] and B [N, K / 2] codes with scale tiles as in mxfp4.cu, fp32
 // accumulation, one rounding to the output type.
 //
-// 64 x 64 tile per block, 4 x 4 outputs per thread, K in steps of one block of
-// 32, decoded into shared memory as fp32 once per tile.  A block's sum of
-// products of elements is exact (multiples of 1/4 up to 1152) and takes both
-// scales at once, so that no factor leaves fp32's range before the product does.
+// Persistent tcgen05 kernel, one CTA per SM, 128 x BN tiles of C:
+//   * codes are read as bytes by TMA, 256 elements of K (one 128-byte swizzle
+//     row) per stage, both operands K-major; scale tiles (512 bytes per 128
+//     rows x 4 blocks, already in the order of TMEM) by untiled bulk copies;
+//   * per stage the MMA thread copies the scales to TMEM and issues up to four
+//     K = 64 MMAs (kind::mxf4).  TMEM holds one scale area per stage of the
+//     ring, so a stage's scales are overwritten only when its barrier has shown
+//     that the MMAs which read them are done;
+//   * two accumulators, so that a tile's read-out overlaps the next tile's
+//     MMAs.  At BN = 256 they and the scales do not fit into the 512 columns
+//     side by side: they overlap by 96 columns, which each read-out empties
+//     first (accumulator 0 from its top, 1 from its bottom).
+// A block of zeros pads K (TMA zero fill); MMAs stop at the last 64 elements
+// that exist.  Rows beyond M or N may multiply stale scales, and are not stored.
+#include <type_traits>
+
 #include "common.h"
-#include "mxfp4.cuh"
+#include "gemm_internal.h"
+#include "sm100.cuh"
+#include "tmap.h"
 #include "vec.cuh"
 
 namespace aotk {
 namespace {
 
-constexpr int kTile = 64;
+using namespace sm100;
 
-// Row r, block j of a scale array.
-__device__ __forceinline__ uint32_t scale_at(const uint8_t* s, int64_t r, int64_t j, int tiles_k) {
-  return s[((r / 128) * tiles_k + j / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + j % 4];
+__device__ unsigned g_mx_watchdog;
+
+constexpr int kBM = 128;
+constexpr int kBK = 256;       // elements of K per stage (128 bytes of codes)
+constexpr int kStepK = 64;     // elements of K per MMA
+constexpr int kThreads = 192;  // producer, MMA and 4 epilogue warps
+constexpr int kGroupM = 16;    // M tiles per raster group
+constexpr uint32_t kScaleTile = 512;
+
+enum : unsigned { kWdProducer = 4096u, kWdMma = 8192u, kWdEpilogue = 16384u };
+
+template <int BN, int STAGES>
+struct MxLayout {
+  static constexpr int kScaleTilesN = BN > 128 ? 2 : 1;  // scale tiles along N
+  static constexpr uint32_t kABytes = kBM * 128;
+  static constexpr uint32_t kBBytes = BN * 128;
+  static constexpr uint32_t kSfaBytes = 2 * kScaleTile;
+  static constexpr uint32_t kSfbBytes = kScaleTilesN * 2 * kScaleTile;
+  static constexpr uint32_t kOffA = 0;
+  static constexpr uint32_t kOffB = kOffA + STAGES * kABytes;
+  static constexpr uint32_t kOffSfa = kOffB + STAGES * kBBytes;
+  static constexpr uint32_t kOffSfb = kOffSfa + STAGES * kSfaBytes;
+  static constexpr uint32_t kCBuf = 32 * 128;
+  static constexpr uint32_t kOffC = kOffSfb + STAGES * kSfbBytes;
+  static constexpr uint32_t kOffBar = kOffC + 4 * kCBuf;
+  static constexpr uint32_t kNumBars = 2 * STAGES + 5;  // full, empty, tfull x2, release x2, drain
+  static constexpr uint32_t kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr uint32_t kAlloc = kOffMisc + 16 + 1024;
+  static_assert(kAlloc <= 232448, "227 KB of shared memory");
+  // TMEM columns: accumulators, then 4 columns per scale tile and stage.
+  static constexpr int kSfCols = 2 * 4 * (1 + kScaleTilesN);
+  static constexpr bool kOverlap = 2 * BN + STAGES * kSfCols > 512;
+  static constexpr int kSfBase = kOverlap ? 512 - STAGES * kSfCols : 2 * BN;
+  static constexpr int kAcc1 = kOverlap ? kSfBase - BN : BN;
+  static constexpr int kShared = BN - kAcc1;  // columns of both accumulators
+  static constexpr int kTmemCols = kSfBase + STAGES * kSfCols > 256 ? 512 : 256;
+  static_assert(kSfBase + STAGES * kSfCols <= kTmemCols, "TMEM columns");
+};
+
+__device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, int& mb, int& nb) {
+  const int per_group = kGroupM * tiles_n;
+  const int g = tile / per_group;
+  const int first_m = g * kGroupM;
+  const int gm = min(tiles_m - first_m, kGroupM);
+  const int local = tile - g * per_group;
+  mb = first_m + local % gm;
+  nb = local / gm;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256)
-    gemm_mxfp4_simt_kernel(T* __restrict__ c, const uint8_t* __restrict__ a,
-                           const uint8_t* __restrict__ as, const uint8_t* __restrict__ b,
-                           const uint8_t* __restrict__ bs, int64_t M, int64_t N, int64_t K,
-                           int tiles_k) {
-  __shared__ float sa[kTile][33], sb[kTile][33];
-  __shared__ int ea[kTile], eb[kTile];  // exponents of the block's scales
-  constexpr int kNan = 1 << 20;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int r = threadIdx.x / 4, q = threadIdx.x % 4;  // row and 8-element word of a block
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += 32) {
-    float va[8] = {}, vb[8] = {};
-    uint32_t xa = 127, xb = 127;
-    if (m0 + r < M) {
-      mx::decode_e2m1x8(*reinterpret_cast<const uint32_t*>(a + ((m0 + r) * K + k0) / 2 + q * 4), va);
-      xa = scale_at(as, m0 + r, k0 / 32, tiles_k);
+__device__ __forceinline__ uint32_t pack_word(const uint32_t* r, int i) {
+  if constexpr (std::is_same_v<T, float>)
+    return r[i];
+  else
+    return Elem<T>::pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+}
+
+template <typename T, int BN, int STAGES>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
+                      const __grid_constant__ CUtensorMap tmB,
+                      const __grid_constant__ CUtensorMap tmC, const uint8_t* __restrict__ a_scales,
+                      const uint8_t* __restrict__ b_scales, T* __restrict__ c, int M, int N, int K,
+                      int tma_store) {
+  using L = MxLayout<BN, STAGES>;
+  constexpr int kChunk = 128 / sizeof(T);  // output columns per staged box
+  constexpr int kChunks = BN / kChunk;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_addr(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const uint32_t bar0 = base + L::kOffBar;
+  const uint32_t drain_bar = bar0 + 8u * (2 * STAGES + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
+  unsigned* wd = &g_mx_watchdog;
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
+  auto release_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int tiles_m = (M + kBM - 1) / kBM;
+  const int tiles_n = (N + BN - 1) / BN;
+  const int num_tiles = tiles_m * tiles_n;
+  const int kblocks = (K + kBK - 1) / kBK;
+  const int sf_tiles_k = (K + 127) / 128;
+  const int sf_tiles_n = (N + 127) / 128;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
     }
-    if (n0 + r < N) {
-      mx::decode_e2m1x8(*reinterpret_cast<const uint32_t*>(b + ((n0 + r) * K + k0) / 2 + q * 4), vb);
-      xb = scale_at(bs, n0 + r, k0 / 32, tiles_k);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(release_bar(a), 4);  // the epilogue warps
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sa[r][q * 8 + i] = va[i];
-      sb[r][q * 8 + i] = vb[i];
-    }
-    if (q == 0) {
-      ea[r] = xa == 255 ? kNan : static_cast<int>(xa) - 127;
-      eb[r] = xb == 255 ? kNan : static_cast<int>(xb) - 127;
-    }
-    __syncthreads();
-    float sum[4][4] = {};
-#pragma unroll 8
-    for (int k = 0; k < 32; ++k) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          sum[i][j] = fmaf(sa[ty + 16 * i][k], sb[tx + 16 * j][k], sum[i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = ea[ty + 16 * i] + eb[tx + 16 * j];
-        acc[i][j] += e >= kNan / 2 ? __int_as_float(0x7FC00000) : ldexpf(sum[i][j], e);
-      }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < M && n < N) c[m * N + n] = Elem<T>::from_f(acc[i][j]);
+  if (warp == 1) {
+    tmem_alloc(smem_addr(tmem_slot), L::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // Global memory is touched only from here on, once the previous kernel on
+  // the stream has completed (programmatic dependent launch).
+  pdl_wait_prior();
+
+  if (warp == 0) {
+    // ---------------- producer ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+        int mb, nb;
+        tile_coords(tile, tiles_m, tiles_n, mb, nb);
+        const int sn0 = nb * BN / 128;  // first scale tile along N
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, wd, kWdProducer)) {
+            ok = false;
+            break;
+          }
+          // Both scale tiles of the K block are neighbours in memory; the
+          // last block may have one, the last N tile too.
+          const int sk = 2 * kb;
+          const uint32_t sf_bytes = (sk + 1 < sf_tiles_k ? 2 : 1) * kScaleTile;
+          const bool second = L::kScaleTilesN == 2 && sn0 + 1 < sf_tiles_n;
+          const uint32_t fb = full_bar(stage);
+          mbar_arrive_expect_tx(fb, L::kABytes + L::kBBytes + (second ? 3 : 2) * sf_bytes);
+          tma_load_2d(base + L::kOffA + stage * L::kABytes, &tmA, kb * 128, mb * kBM, fb);
+          tma_load_2d(base + L::kOffB + stage * L::kBBytes, &tmB, kb * 128, nb * BN, fb);
+          bulk_load(base + L::kOffSfa + stage * L::kSfaBytes,
+                    a_scales + (static_cast<int64_t>(mb) * sf_tiles_k + sk) * kScaleTile, sf_bytes,
+                    fb);
+          const uint8_t* sb = b_scales + (static_cast<int64_t>(sn0) * sf_tiles_k + sk) * kScaleTile;
+          const uint32_t sfb = base + L::kOffSfb + stage * L::kSfbBytes;
+          bulk_load(sfb, sb, sf_bytes, fb);
+          if (second)
+            bulk_load(sfb + 2 * kScaleTile, sb + static_cast<int64_t>(sf_tiles_k) * kScaleTile,
+                      sf_bytes, fb);
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      int s = stage;
+      uint32_t p = phase;
+      for (int i = 0; i < STAGES && i < issued; ++i) {
+        if (--s < 0) {
+          s = STAGES - 1;
+          p ^= 1u;
+        }
+        mbar_drain(full_bar(s), p);
+      }
     }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;  // tiles of this CTA
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x, ++it) {
+        int mb, nb;
+        tile_coords(tile, tiles_m, tiles_n, mb, nb);
+        const int acc = it & 1;
+        // Overlapping accumulators: the previous tile's read-out has left the
+        // shared columns.  Else: the read-out before it has left this one.
+        const int need = L::kOverlap ? it - 1 : it - 2;
+        if (need >= 0 &&
+            !mbar_wait_bounded(release_bar(L::kOverlap ? 0 : acc),
+                               (L::kOverlap ? need : need >> 1) & 1, abort_flag, wd, kWdMma)) {
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (acc ? L::kAcc1 : 0);
+        // A 64-column tile may be the upper half of its scale tile: 2 columns on.
+        const uint32_t sfb_shift = BN == 64 ? (nb & 1) * 2 : 0;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, wd, kWdMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sfa = tmem_base + L::kSfBase + stage * L::kSfCols;
+          const uint32_t sfb = sfa + 8;
+          const uint32_t sa = base + L::kOffSfa + stage * L::kSfaBytes;
+          const uint32_t sb = base + L::kOffSfb + stage * L::kSfbBytes;
+          const uint32_t a0 = base + L::kOffA + stage * L::kABytes;
+          const uint32_t b0 = base + L::kOffB + stage * L::kBBytes;
+          const int steps = min(kBK / kStepK, (K - kb * kBK + kStepK - 1) / kStepK);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {  // halves of 128 elements: one scale tile each
+            if (2 * t < steps) {
+              tmem_cp_scales(sfa + 4 * t, sdesc_scales(sa + t * kScaleTile));
+#pragma unroll
+              for (int j = 0; j < L::kScaleTilesN; ++j)
+                tmem_cp_scales(sfb + 4 * (L::kScaleTilesN * t + j),
+                               sdesc_scales(sb + (2 * j + t) * kScaleTile));
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int k = 2 * t + h;
+                if (k < steps)
+                  umma_mxf4(d_tmem, sdesc_sw128(a0 + k * 32, 16, 1024),
+                            sdesc_sw128(b0 + k * 32, 16, 1024), idesc_mxf4(kBM, BN, 2 * h),
+                            sfa + 4 * t, sfb + 4 * L::kScaleTilesN * t + sfb_shift,
+                            kb > 0 || k > 0);
+              }
+            }
+          }
+          umma_commit(empty_bar(stage));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        umma_commit(tfull_bar(acc));
+      }
+      umma_commit(drain_bar);
+      mbar_drain(drain_bar, 0);
+    }
+    __syncwarp();
+  } else {
+    // ---------------- epilogue (warps 2..5) ----------------
+    const int q = warp & 3;
+    const uint32_t buf = base + L::kOffC + (warp - 2) * L::kCBuf;
+    uint8_t* buf_ptr = smem + L::kOffC + (warp - 2) * L::kCBuf;
+    int it = 0;
+    bool stored = false;
+    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++it) {
+      int mb, nb;
+      tile_coords(tile, tiles_m, tiles_n, mb, nb);
+      const int acc = it & 1;
+      int ok = 1;
+      if (lane == 0)
+        ok = mbar_wait_bounded(tfull_bar(acc), (it >> 1) & 1, abort_flag, wd, kWdEpilogue);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t trow = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (acc ? L::kAcc1 : 0);
+      const int y = mb * kBM + q * 32;
+      // Chunks after which the columns of both accumulators have been read.
+      constexpr int kRelease = L::kOverlap ? (L::kShared + kChunk - 1) / kChunk : kChunks;
+#pragma unroll 1
+      for (int i = 0; i < kChunks; ++i) {
+        const int ch = L::kOverlap && acc == 0 ? kChunks - 1 - i : i;
+        uint32_t r[kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; j += 32) tmem_ld_32x32b_x32(trow + ch * kChunk + j, r + j);
+        tmem_wait_ld();
+        if (i == kRelease - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(release_bar(L::kOverlap ? 0 : acc));
+        }
+        const int x = nb * BN + ch * kChunk;
+        if (x >= N || y >= M) continue;
+        if (stored && tma_store && lane == 0) bulk_wait_read<0>();
+        __syncwarp();
+        const uint32_t srow = buf + lane * 128;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          st_shared_v4(srow + ((j ^ (lane & 7)) << 4), pack_word<T>(r, 4 * j),
+                       pack_word<T>(r, 4 * j + 1), pack_word<T>(r, 4 * j + 2),
+                       pack_word<T>(r, 4 * j + 3));
+        if (tma_store) {
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC, buf, x, y);
+            bulk_commit();
+          }
+          stored = true;
+        } else {
+          // Row strides or a base that TMA cannot address: element stores, a
+          // row at a time.
+          __syncwarp();
+          const int rows = min(32, M - y);
+          for (int rr = 0; rr < rows; ++rr) {
+            T* crow = c + static_cast<int64_t>(y + rr) * N + x;
+#pragma unroll
+            for (int e = lane; e < kChunk; e += 32) {
+              const int b = e * static_cast<int>(sizeof(T));
+              const T v = *reinterpret_cast<const T*>(
+                  buf_ptr + rr * 128 + (((b >> 4) ^ (rr & 7)) << 4) + (b & 15));
+              if (x + e < N) crow[e] = v;
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::kTmemCols);
+  }
 }
 
 template <typename T>
-int launch(void* c, const void* a, const void* as, const void* b, const void* bs, int64_t M,
-           int64_t N, int64_t K, cudaStream_t s) {
-  const int64_t gy = (M + kTile - 1) / kTile;
-  if (gy > 65535) return fail(AOTK_ERR_UNSUPPORTED, "aotk_mxfp4_gemm: M = %lld", (long long)M);
-  const dim3 grid(static_cast<unsigned>((N + kTile - 1) / kTile), static_cast<unsigned>(gy));
-  gemm_mxfp4_simt_kernel<T><<<grid, 256, 0, s>>>(
-      static_cast<T*>(c), static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(as),
-      static_cast<const uint8_t*>(b), static_cast<const uint8_t*>(bs), M, N, K,
-      static_cast<int>((K + 127) / 128));
+int output_map(CUtensorMap* tm, const void* c, int M, int N, int* tma_store) {
+  *tma_store = aligned16(c) && static_cast<int64_t>(N) * sizeof(T) % 16 == 0;
+  if (!*tma_store) return AOTK_OK;
+  if constexpr (std::is_same_v<T, float>)
+    return make_tmap_2d_f32(tm, c, M, N, N, 32, 32);
+  else
+    return make_tmap_2d_16bit(tm, c, std::is_same_v<T, __nv_bfloat16>, M, N, N, 64, 32);
+}
+
+template <typename T, int BN, int STAGES>
+int launch_tiles(void* c, const void* a, const void* as, const void* b, const void* bs, int M,
+                 int N, int K, cudaStream_t stream, const DeviceInfo& info) {
+  using L = MxLayout<BN, STAGES>;
+  auto kernel = gemm_mxfp4_kernel<T, BN, STAGES>;
+  if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, info)) return st;
+  CUtensorMap ta, tb, tc = {};
+  int tma_store = 0;
+  if (int st = make_tmap_2d_8bit(&ta, a, M, K / 2, K / 2, 128, kBM)) return st;
+  if (int st = make_tmap_2d_8bit(&tb, b, N, K / 2, K / 2, 128, BN)) return st;
+  if (int st = output_map<T>(&tc, c, M, N, &tma_store)) return st;
+  const int64_t tiles = static_cast<int64_t>((M + kBM - 1) / kBM) * ((N + BN - 1) / BN);
+  if (tiles > 0x7fffffffLL)
+    return fail(AOTK_ERR_UNSUPPORTED, "aotk_mxfp4_gemm: output of %d x %d has too many tiles", M, N);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles < info.sm_count ? tiles : info.sm_count), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kAlloc;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(
+      &cfg, kernel, ta, tb, tc, static_cast<const uint8_t*>(as), static_cast<const uint8_t*>(bs),
+      static_cast<T*>(c), M, N, K, tma_store);
+  if (e != cudaSuccess)
+    return fail(AOTK_ERR_CUDA, "aotk_mxfp4_gemm launch: %s", cudaGetErrorString(e));
   return check_launch("aotk_mxfp4_gemm");
 }
 
+template <typename T>
+int dispatch(void* c, const void* a, const void* as, const void* b, const void* bs, int M, int N,
+             int K, cudaStream_t s) {
+  DeviceInfo info;
+  if (int st = current_device_info(&info)) return st;
+  if (int st = require_sm100(info)) return st;
+  // Rounds of tiles on the SMs, in units of 256 columns.
+  auto rounds = [&](int bn) {
+    const int64_t tiles = static_cast<int64_t>((M + kBM - 1) / kBM) * ((N + bn - 1) / bn);
+    return static_cast<double>((tiles + info.sm_count - 1) / info.sm_count) * bn / 256;
+  };
+  const double r256 = rounds(256), r128 = 1.1 * rounds(128), r64 = 1.3 * rounds(64);
+  if (r256 <= r128 && r256 <= r64)
+    return launch_tiles<T, 256, 4>(c, a, as, b, bs, M, N, K, s, info);
+  if (r128 <= r64) return launch_tiles<T, 128, 6>(c, a, as, b, bs, M, N, K, s, info);
+  return launch_tiles<T, 64, 7>(c, a, as, b, bs, M, N, K, s, info);
+}
+
 }  // namespace
+
+int mxfp4_watchdog(uint32_t* status, bool clear) {
+  unsigned v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_mx_watchdog, sizeof(v));
+  if (e != cudaSuccess) return fail(AOTK_ERR_CUDA, "watchdog read: %s", cudaGetErrorString(e));
+  if (clear) {
+    const unsigned zero = 0;
+    e = cudaMemcpyToSymbol(g_mx_watchdog, &zero, sizeof(zero));
+    if (e != cudaSuccess) return fail(AOTK_ERR_CUDA, "watchdog clear: %s", cudaGetErrorString(e));
+  }
+  *status |= v;
+  return AOTK_OK;
+}
+
 }  // namespace aotk
 
 extern "C" int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, const void* b,
@@ -122,9 +450,10 @@ extern "C" int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, con
   }
   if (!aligned16(a) || !aligned16(b) || !aligned16(a_scales) || !aligned16(b_scales))
     return fail(AOTK_ERR_UNSUPPORTED, "%s: codes and scales must be 16-byte aligned", who);
+  const int m = (int)M, n = (int)N, k = (int)K;
   switch (out_dtype) {
-    case AOTK_FLOAT32: return launch<float>(c, a, a_scales, b, b_scales, M, N, K, s);
-    case AOTK_FLOAT16: return launch<__half>(c, a, a_scales, b, b_scales, M, N, K, s);
-    default: return launch<__nv_bfloat16>(c, a, a_scales, b, b_scales, M, N, K, s);
+    case AOTK_FLOAT32: return dispatch<float>(c, a, a_scales, b, b_scales, m, n, k, s);
+    case AOTK_FLOAT16: return dispatch<__half>(c, a, a_scales, b, b_scales, m, n, k, s);
+    default: return dispatch<__nv_bfloat16>(c, a, a_scales, b, b_scales, m, n, k, s);
   }
 }

@@ -135,6 +135,17 @@ __device__ __forceinline__ void tma_store_2d_hint(const CUtensorMap* map, uint32
       : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16) from 16-byte aligned global memory,
+// counted on `bar` like a tiled load.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
 __device__ __forceinline__ void bulk_commit() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
@@ -207,6 +218,30 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
       : "memory");
+}
+
+// D[tmem] (+)= A * B of packed e2m1 operands (64 elements of K per step), each
+// block of 32 along K multiplied by 2^(byte - 127) for its row of A and of B.
+// A word of scales (four blocks, two steps) is one TMEM column of 32 lanes per
+// 32 rows; the instruction descriptor names the pair of bytes that is meant.
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                          bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+// Copies one 512-byte tile of scales (32 rows of 16 bytes) to 4 TMEM columns,
+// repeated in all four 32-lane quarters.  Ordered before the MMAs that this
+// thread issues after it.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t s_desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc)
+               : "memory");
 }
 
 // Arrives once on `bar` when every tcgen05.mma issued so far by this thread
@@ -328,6 +363,16 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr, uint32_t lbo_byt
   return d;
 }
 
+// Shared-memory matrix descriptor of a tile of scales: no swizzle, 8-row groups
+// of 16-byte rows 128 bytes apart.
+__device__ __forceinline__ uint64_t sdesc_scales(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128u >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+
 // Instruction descriptor for kind::f16 with fp32 accumulation:
 //   bits [4,6) D format (1 = f32), [7,10) A format, [10,13) B format
 //   (0 = f16, 1 = bf16), bit 15 A major, bit 16 B major (0 = K, 1 = MN),
@@ -347,6 +392,16 @@ __host__ __device__ constexpr uint32_t idesc_make(uint32_t c_fmt, uint32_t ab_fm
   return (c_fmt << 4) | (ab_fmt << 7) | (ab_fmt << 10) | ((a_mn_major ? 1u : 0u) << 15) |
          ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Instruction descriptor for kind::mxf4 (fp32 accumulation, both operands
+// K-major): bits [4,6) scale id of B, [7,10) A and [10,13) B format (1 = e2m1),
+// [17,23) N >> 3, bit 23 scale format (1 = power of two), [24,29) M >> 4,
+// [29,31) scale id of A.  A scale id (0 or 2) is the first byte of the pair
+// that the step uses.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, uint32_t scale_id) {
+  return (scale_id << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) | (scale_id << 29);
 }
 
 // ---- programmatic dependent launch ---------------------------------------------
