@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
   auto release_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform
   const int lane = threadIdx.x & 31;
   const int tiles_m = (M + kBM - 1) / kBM;
   const int tiles_n = (N + BN - 1) / BN;
@@ -149,45 +149,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ---------------- producer ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int issued = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
-        int mb, nb;
-        tile_coords(tile, tiles_m, tiles_n, mb, nb);
-        const int sn0 = nb * BN / 128;  // first scale tile along N
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, wd, kWdProducer)) {
-            ok = false;
-            break;
-          }
-          // Both scale tiles of the K block are neighbours in memory; the
-          // last block may have one, the last N tile too.
-          const int sk = 2 * kb;
-          const uint32_t sf_bytes = (sk + 1 < sf_tiles_k ? 2 : 1) * kScaleTile;
-          const bool second = L::kScaleTilesN == 2 && sn0 + 1 < sf_tiles_n;
-          const uint32_t fb = full_bar(stage);
+    const bool elected = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+      int mb, nb;
+      tile_coords(tile, tiles_m, tiles_n, mb, nb);
+      const int sn0 = nb * BN / 128;  // first scale tile along N
+      const bool second = L::kScaleTilesN == 2 && sn0 + 1 < sf_tiles_n;
+      const uint8_t* sfa_row = a_scales + static_cast<int64_t>(mb) * sf_tiles_k * kScaleTile;
+      const uint8_t* sfb_row = b_scales + static_cast<int64_t>(sn0) * sf_tiles_k * kScaleTile;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, wd, kWdProducer);
+        if (!ok) break;
+        // Both scale tiles of the K block are neighbours in memory; the last
+        // block may have one, the last N tile too.
+        const int sk = 2 * kb;
+        const uint32_t sf_bytes = (sk + 1 < sf_tiles_k ? 2 : 1) * kScaleTile;
+        const uint32_t fb = full_bar(stage);
+        const uint32_t sfb = base + L::kOffSfb + stage * L::kSfbBytes;
+        if (elected) {
           mbar_arrive_expect_tx(fb, L::kABytes + L::kBBytes + (second ? 3 : 2) * sf_bytes);
           tma_load_2d(base + L::kOffA + stage * L::kABytes, &tmA, kb * 128, mb * kBM, fb);
           tma_load_2d(base + L::kOffB + stage * L::kBBytes, &tmB, kb * 128, nb * BN, fb);
-          bulk_load(base + L::kOffSfa + stage * L::kSfaBytes,
-                    a_scales + (static_cast<int64_t>(mb) * sf_tiles_k + sk) * kScaleTile, sf_bytes,
+          bulk_load(base + L::kOffSfa + stage * L::kSfaBytes, sfa_row + sk * kScaleTile, sf_bytes,
                     fb);
-          const uint8_t* sb = b_scales + (static_cast<int64_t>(sn0) * sf_tiles_k + sk) * kScaleTile;
-          const uint32_t sfb = base + L::kOffSfb + stage * L::kSfbBytes;
-          bulk_load(sfb, sb, sf_bytes, fb);
+          bulk_load(sfb, sfb_row + sk * kScaleTile, sf_bytes, fb);
           if (second)
-            bulk_load(sfb + 2 * kScaleTile, sb + static_cast<int64_t>(sf_tiles_k) * kScaleTile,
-                      sf_bytes, fb);
-          ++issued;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+            bulk_load(sfb + 2 * kScaleTile,
+                      sfb_row + (static_cast<int64_t>(sf_tiles_k) + sk) * kScaleTile, sf_bytes, fb);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
+    }
+    if (elected) {
       int s = stage;
       uint32_t p = phase;
       for (int i = 0; i < STAGES && i < issued; ++i) {
@@ -201,68 +203,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int it = 0;  // tiles of this CTA
-      bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x, ++it) {
-        int mb, nb;
-        tile_coords(tile, tiles_m, tiles_n, mb, nb);
-        const int acc = it & 1;
-        // Overlapping accumulators: the previous tile's read-out has left the
-        // shared columns.  Else: the read-out before it has left this one.
-        const int need = L::kOverlap ? it - 1 : it - 2;
-        if (need >= 0 &&
-            !mbar_wait_bounded(release_bar(L::kOverlap ? 0 : acc),
-                               (L::kOverlap ? need : need >> 1) & 1, abort_flag, wd, kWdMma)) {
-          break;
-        }
+    const bool elected = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    int it = 0;  // tiles of this CTA
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x, ++it) {
+      int mb, nb;
+      tile_coords(tile, tiles_m, tiles_n, mb, nb);
+      const int acc = it & 1;
+      // Overlapping accumulators: the previous tile's read-out has left the
+      // shared columns.  Else: the read-out before it has left this one.
+      const int need = L::kOverlap ? it - 1 : it - 2;
+      if (need >= 0) {
+        ok = mbar_wait_warp(release_bar(L::kOverlap ? 0 : acc),
+                            (L::kOverlap ? need : need >> 1) & 1, abort_flag, wd, kWdMma);
+        if (!ok) break;
+      }
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + (acc ? L::kAcc1 : 0);
+      // A 64-column tile may be the upper half of its scale tile: 2 columns on.
+      const uint32_t sfb_shift = BN == 64 ? (nb & 1) * 2 : 0;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        ok = mbar_wait_warp(full_bar(stage), phase, abort_flag, wd, kWdMma);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (acc ? L::kAcc1 : 0);
-        // A 64-column tile may be the upper half of its scale tile: 2 columns on.
-        const uint32_t sfb_shift = BN == 64 ? (nb & 1) * 2 : 0;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, wd, kWdMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sfa = tmem_base + L::kSfBase + stage * L::kSfCols;
-          const uint32_t sfb = sfa + 8;
-          const uint32_t sa = base + L::kOffSfa + stage * L::kSfaBytes;
-          const uint32_t sb = base + L::kOffSfb + stage * L::kSfbBytes;
-          const uint32_t a0 = base + L::kOffA + stage * L::kABytes;
-          const uint32_t b0 = base + L::kOffB + stage * L::kBBytes;
-          const int steps = min(kBK / kStepK, (K - kb * kBK + kStepK - 1) / kStepK);
+        const uint32_t sfa = tmem_base + L::kSfBase + stage * L::kSfCols;
+        const uint32_t sfb = sfa + 8;
+        const uint64_t sa = sdesc_scales(base + L::kOffSfa + stage * L::kSfaBytes);
+        const uint64_t sb = sdesc_scales(base + L::kOffSfb + stage * L::kSfbBytes);
+        const uint64_t ad = sdesc_sw128(base + L::kOffA + stage * L::kABytes, 16, 1024);
+        const uint64_t bd = sdesc_sw128(base + L::kOffB + stage * L::kBBytes, 16, 1024);
+        const int steps = min(kBK / kStepK, (K - kb * kBK + kStepK - 1) / kStepK);
+        if (elected) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {  // halves of 128 elements: one scale tile each
             if (2 * t < steps) {
-              tmem_cp_scales(sfa + 4 * t, sdesc_scales(sa + t * kScaleTile));
+              // Descriptors count addresses in units of 16 bytes.
+              tmem_cp_scales(sfa + 4 * t, sa + t * (kScaleTile / 16));
 #pragma unroll
               for (int j = 0; j < L::kScaleTilesN; ++j)
                 tmem_cp_scales(sfb + 4 * (L::kScaleTilesN * t + j),
-                               sdesc_scales(sb + (2 * j + t) * kScaleTile));
+                               sb + (2 * j + t) * (kScaleTile / 16));
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int k = 2 * t + h;
                 if (k < steps)
-                  umma_mxf4(d_tmem, sdesc_sw128(a0 + k * 32, 16, 1024),
-                            sdesc_sw128(b0 + k * 32, 16, 1024), idesc_mxf4(kBM, BN, 2 * h),
-                            sfa + 4 * t, sfb + 4 * L::kScaleTilesN * t + sfb_shift,
-                            kb > 0 || k > 0);
+                  umma_mxf4(d_tmem, ad + k * 2, bd + k * 2, idesc_mxf4(kBM, BN, 2 * h), sfa + 4 * t,
+                            sfb + 4 * L::kScaleTilesN * t + sfb_shift, kb > 0 || k > 0);
               }
             }
           }
           umma_commit(empty_bar(stage));
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
         }
-        if (!ok) break;
-        umma_commit(tfull_bar(acc));
+        __syncwarp();
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
+      if (!ok) break;
+      if (elected) umma_commit(tfull_bar(acc));
+      __syncwarp();
+    }
+    if (elected) {
       umma_commit(drain_bar);
       mbar_drain(drain_bar, 0);
     }

@@ -81,6 +81,27 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   }
 }
 
+// One lane of the (converged) warp gets true.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+
+// mbar_wait_bounded by a whole converged warp, which stays converged: the
+// result comes from a vote, so the compiler may keep what the warp computes in
+// uniform registers - where the operands of tcgen05 and TMA instructions have
+// to be - instead of moving each of them there from one lane's.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort,
+                                               unsigned* status, unsigned code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, status, code));
+}
+
 // Same bound, ignoring the abort flag: used only to drain copies that are
 // already in flight before a CTA exits.
 __device__ __forceinline__ bool mbar_drain(uint32_t bar, uint32_t parity) {
