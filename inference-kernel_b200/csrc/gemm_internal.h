@@ -73,6 +73,17 @@ constexpr int64_t kSkinnyMaxM = 128;
 int gemm_skinny(void* c, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int dtype,
                 void* stream);
 
+// Clusters of `cs` 192-thread CTAs with `smem` bytes each that can be resident
+// at once on the device, for kernels whose TMEM lets two CTAs share an SM
+// (gemm_skinny.cu).
+int resident_clusters(int cs, int smem, const DeviceInfo& info, int* out);
+
+// 4-bit product for M <= kSkinnyMaxM (gemm_mxfp4_skinny.cu); arguments checked
+// by aotk_mxfp4_gemm.
+int gemm_mxfp4_skinny(void* c, const void* a, const void* a_scales, const void* b,
+                      const void* b_scales, int M, int N, int K, int out_dtype, void* stream,
+                      const DeviceInfo& info);
+
 // SIMT kernel for every dtype and shape (gemm_simt.cu).
 int gemm_simt(void* c, const void* a, const void* b, int64_t M, int64_t N, int64_t K, int dtype,
               void* stream);
@@ -83,6 +94,7 @@ int watchdog_selftest(void* stream);
 // Watchdog words of the tensor-core kernels (OR-ed into *status).
 int tc_watchdog(uint32_t* status, bool clear);
 int mxfp4_watchdog(uint32_t* status, bool clear);
+int mxfp4_skinny_watchdog(uint32_t* status, bool clear);
 int skinny_watchdog(uint32_t* status, bool clear);
 
 // Raises the dynamic shared-memory limit of `kernel` to `bytes` once per device.

@@ -397,10 +397,7 @@ int launch_tiles(void* c, const void* a, const void* as, const void* b, const vo
 
 template <typename T>
 int dispatch(void* c, const void* a, const void* as, const void* b, const void* bs, int M, int N,
-             int K, cudaStream_t s) {
-  DeviceInfo info;
-  if (int st = current_device_info(&info)) return st;
-  if (int st = require_sm100(info)) return st;
+             int K, cudaStream_t s, const DeviceInfo& info) {
   // Rounds of tiles on the SMs, in units of 256 columns.
   auto rounds = [&](int bn) {
     const int64_t tiles = static_cast<int64_t>((M + kBM - 1) / kBM) * ((N + bn - 1) / bn);
@@ -454,10 +451,15 @@ extern "C" int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, con
   }
   if (!aligned16(a) || !aligned16(b) || !aligned16(a_scales) || !aligned16(b_scales))
     return fail(AOTK_ERR_UNSUPPORTED, "%s: codes and scales must be 16-byte aligned", who);
+  DeviceInfo info;
+  if (int st = current_device_info(&info)) return st;
+  if (int st = require_sm100(info)) return st;
   const int m = (int)M, n = (int)N, k = (int)K;
+  if (M <= kSkinnyMaxM)
+    return gemm_mxfp4_skinny(c, a, a_scales, b, b_scales, m, n, k, out_dtype, stream, info);
   switch (out_dtype) {
-    case AOTK_FLOAT32: return dispatch<float>(c, a, a_scales, b, b_scales, m, n, k, s);
-    case AOTK_FLOAT16: return dispatch<__half>(c, a, a_scales, b, b_scales, m, n, k, s);
-    default: return dispatch<__nv_bfloat16>(c, a, a_scales, b, b_scales, m, n, k, s);
+    case AOTK_FLOAT32: return dispatch<float>(c, a, a_scales, b, b_scales, m, n, k, s, info);
+    case AOTK_FLOAT16: return dispatch<__half>(c, a, a_scales, b, b_scales, m, n, k, s, info);
+    default: return dispatch<__nv_bfloat16>(c, a, a_scales, b, b_scales, m, n, k, s, info);
   }
 }

@@ -250,6 +250,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 // an SM when shared memory allows, and clusters pack accordingly.
 __global__ void __launch_bounds__(kThreads, 2) skinny_shadow_kernel() {}
 
+}  // namespace
+
 // Clusters of `cs` skinny CTAs with `smem` bytes each that can be resident at
 // once on the device (cached per device, cluster size and shared-memory size).
 int resident_clusters(int cs, int smem, const DeviceInfo& info, int* out) {
@@ -266,7 +268,10 @@ int resident_clusters(int cs, int smem, const DeviceInfo& info, int* out) {
       return AOTK_OK;
     }
   }
-  if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(skinny_shadow_kernel), smem, info))
+  // The limit is set once per kernel and device, so to the most that any caller
+  // may ask for: a query above a smaller limit finds no room for any cluster.
+  if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(skinny_shadow_kernel),
+                                   info.max_smem_optin, info))
     return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(cs), 1, 1);
@@ -288,6 +293,8 @@ int resident_clusters(int cs, int smem, const DeviceInfo& info, int* out) {
   *out = n;
   return AOTK_OK;
 }
+
+namespace {
 
 template <typename T, int MP, int STAGES>
 int launch_skinny(void* c, const void* a, const void* b, int M, int N, int K, bool bf16,
