@@ -335,6 +335,26 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
+// umma_mxf4 for a CTA pair: M = 256.  Each CTA's TMEM holds the scales of its
+// own 128 rows of A and of all N rows of B.
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t sfa_tmem,
+                                               uint32_t sfb_tmem, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+// tmem_cp_scales in both CTAs of the pair, each from its own shared memory.
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t s_desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc)
+               : "memory");
+}
+
 // Arrives once on the mbarrier at shared offset `bar` in every CTA of `mask`
 // when all prior tcgen05.mma of this thread have completed.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint16_t mask) {

@@ -34,7 +34,8 @@ int encoder(EncodeTiledFn* fn) {
 }
 
 int encode_2d(CUtensorMap* map, CUtensorMapDataType type, uint32_t elem_bytes, const void* base,
-              uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
+              uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows,
+              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn fn;
   if (int st = encoder(&fn)) return st;
   const cuuint64_t dims[2] = {cols, rows};
@@ -42,7 +43,7 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType type, uint32_t elem_bytes, c
   const cuuint32_t box[2] = {box_cols, box_rows};
   const cuuint32_t estrides[2] = {1, 1};
   CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estrides,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(AOTK_ERR_CUDA,
@@ -63,6 +64,11 @@ int make_tmap_2d_8bit(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 int make_tmap_2d_f32(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                      uint32_t box_cols, uint32_t box_rows) {
   return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, rows, cols, ld, box_cols, box_rows);
+}
+
+int make_tmap_blocks512(CUtensorMap* map, const void* base, uint64_t count, uint32_t box_rows) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, base, count, 128, 128, 128, box_rows,
+                   CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 int make_tmap_2d_16bit(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols,

@@ -24,4 +24,8 @@ int make_tmap_2d_8bit(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 int make_tmap_2d_f32(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                      uint32_t box_cols, uint32_t box_rows);
 
+// `count` consecutive blocks of 512 bytes as rows, box = box_rows whole blocks,
+// not swizzled, zeros beyond the last block.
+int make_tmap_blocks512(CUtensorMap* map, const void* base, uint64_t count, uint32_t box_rows);
+
 }  // namespace aotk
