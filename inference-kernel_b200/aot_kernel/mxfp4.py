@@ -17,28 +17,18 @@ has quantised (jit_kernel/gemm.py:199-248).
 import torch
 
 from . import _C  # noqa: F401  (registers torch.ops.aot_kernel.*)
-from .utils import assert_contiguous, assert_is_cuda, assert_same_device
 
 BLOCK = 32
-_FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+# The operators check their arguments and allocate (ValueError; RuntimeError for
+# tensors that are not on a CUDA device).
+_quantize = torch.ops.aot_kernel.mxfp4_quantize.default
+_dequantize = torch.ops.aot_kernel.mxfp4_dequantize.default
+_gemm = torch.ops.aot_kernel.mxfp4_gemm.default
+_gemm_out = torch.ops.aot_kernel.mxfp4_gemm_out.default
 
 
 def _tiles(rows: int, cols: int) -> tuple[int, int, int]:
     return ((rows + 127) // 128, (cols + 127) // 128, 512)
-
-
-def _assert_pair(codes: torch.Tensor, scales: torch.Tensor) -> None:
-    assert_is_cuda(codes, scales)
-    assert_contiguous(codes, scales)
-    assert_same_device(codes, scales)
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise ValueError(f"codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
-    if codes.dim() != 2 or codes.size(1) % (BLOCK // 2):
-        raise ValueError(f"codes must be [rows, cols / 2] with cols a multiple of {BLOCK}, "
-                         f"got {tuple(codes.shape)}")
-    if scales.shape != _tiles(codes.size(0), 2 * codes.size(1)):
-        raise ValueError(f"scales of codes {tuple(codes.shape)} must be "
-                         f"{_tiles(codes.size(0), 2 * codes.size(1))}, got {tuple(scales.shape)}")
 
 
 def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -50,29 +40,13 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     magnitudes above 6 become 6.  A block that holds a NaN or an infinity reads
     back as NaN.
     """
-    assert_is_cuda(x)
-    if x.dtype not in _FLOAT_DTYPES:
-        raise ValueError(f"mxfp4_quantize expects float32, float16 or bfloat16, got {x.dtype}")
-    if x.dim() != 2 or x.size(1) % BLOCK:
-        raise ValueError(f"x must be [rows, cols] with cols a multiple of {BLOCK}, got {tuple(x.shape)}")
-    if not x.is_contiguous() and (x.stride(1) != 1 or x.stride(0) < x.size(1)):
-        raise ValueError("x must be contiguous or a 2-D view with contiguous rows")
-    rows, cols = x.shape
-    codes = torch.empty((rows, cols // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_tiles(rows, cols), dtype=torch.uint8, device=x.device)
-    torch.ops.aot_kernel.mxfp4_quantize(codes, scales, x)
-    return codes, scales
+    return _quantize(x)
 
 
 def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
                      dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [rows, cols] that codes and scales stand for, rounded once to dtype."""
-    _assert_pair(codes, scales)
-    if dtype not in _FLOAT_DTYPES:
-        raise ValueError(f"mxfp4_dequantize gives float32, float16 or bfloat16, not {dtype}")
-    out = torch.empty((codes.size(0), 2 * codes.size(1)), dtype=dtype, device=codes.device)
-    torch.ops.aot_kernel.mxfp4_dequantize(out, codes, scales)
-    return out
+    return _dequantize(codes, scales, dtype)
 
 
 def mxfp4_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
@@ -84,20 +58,11 @@ def mxfp4_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
 
     ``out`` may name a contiguous [M, N] tensor of dtype ``out_dtype`` to write into.
     """
-    _assert_pair(a, a_scales)
-    _assert_pair(b, b_scales)
-    device = assert_same_device(a, b)
-    if a.size(1) != b.size(1):
-        raise ValueError(f"inner dims mismatch: {2 * a.size(1)} vs {2 * b.size(1)}")
-    if out_dtype not in _FLOAT_DTYPES:
-        raise ValueError(f"mxfp4_gemm gives float32, float16 or bfloat16, not {out_dtype}")
-    shape = (a.size(0), b.size(0))
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=device)
-    elif (out.shape != shape or out.dtype != out_dtype or out.device != device
-          or not out.is_contiguous()):
-        raise ValueError(f"out must be a contiguous {out_dtype} tensor {shape} on {device}")
-    torch.ops.aot_kernel.mxfp4_gemm(out, a, a_scales, b, b_scales)
+        return _gemm(a, a_scales, b, b_scales, out_dtype)
+    if out.dtype != out_dtype:
+        raise ValueError(f"out must be {out_dtype}, got {out.dtype}")
+    _gemm_out(out, a, a_scales, b, b_scales)
     return out
 
 

@@ -1,11 +1,11 @@
 """RMSNorm wrapper (reference: aot_kernel/norm.py:9-18)."""
 
-import math
-
 import torch
 
 from . import _C  # noqa: F401  (registers torch.ops.aot_kernel.*)
 from .utils import assert_contiguous, assert_same_device, assert_same_dtype
+
+_sandwich_rmsnorm = torch.ops.aot_kernel.sandwich_rmsnorm.default
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
@@ -43,21 +43,6 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     return out, h
 
 
-def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
-    """``gate`` as [gate_rows, H] or [gate_rows, 1], where gate row i serves the
-    i-th of gate_rows equal runs of x's rows."""
-    if gate.dim() > x.dim() or gate.dim() == 0 or gate.size(-1) not in (1, x.size(-1)):
-        raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over x {tuple(x.shape)}")
-    lead = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape[:-1])
-    i = 0
-    while i < len(lead) and lead[i] == x.shape[i]:
-        i += 1
-    if any(n != 1 for n in lead[i:]):
-        raise ValueError(f"gate {tuple(gate.shape)} must match leading dims of x {tuple(x.shape)} "
-                         "and be 1 in the others")
-    return gate.reshape(math.prod(lead), gate.size(-1))
-
-
 def sandwich_rmsnorm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor,
                      pre_weight: torch.Tensor, eps: float = 1e-6, *,
                      gate: torch.Tensor | None = None,
@@ -72,23 +57,12 @@ def sandwich_rmsnorm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch
     x: its last dim is H or 1, its leading dims match x's from the left and are 1
     after that - e.g. ``[H]`` (per channel), ``[B, 1, H]`` (per sequence),
     ``[B, S, 1]`` (per token) or x's own shape.  A factor on the block's branch
-    can be folded into ``gate`` or ``post_weight``.
+    can be folded into ``gate`` or ``post_weight``.  All tensors are contiguous and of
+    one dtype; anything else is a ValueError.  Forward only, like the other norms.
     """
     if not x.is_cuda:
         raise ValueError("cuda sandwich_rmsnorm requires a CUDA tensor")
-    tensors = [x, residual, post_weight, pre_weight] + ([gate] if gate is not None else [])
-    assert_contiguous(*tensors)
-    assert_same_device(*tensors)
-    assert_same_dtype(*tensors)
-    if x.shape != residual.shape:
-        raise ValueError(f"shape mismatch: x {tuple(x.shape)} vs residual {tuple(residual.shape)}")
-    if gate is not None:
-        gate = _gate_rows(gate, x)
-    out = torch.empty_like(x)
-    h = torch.empty_like(x)
-    torch.ops.aot_kernel.sandwich_rmsnorm(out, h, x, residual, post_weight, pre_weight, gate,
-                                          residual_scale, eps)
-    return out, h
+    return _sandwich_rmsnorm(x, residual, post_weight, pre_weight, gate, residual_scale, eps)
 
 
 def rms_rstd(x: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:

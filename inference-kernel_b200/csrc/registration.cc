@@ -15,6 +15,7 @@
 #include <torch/library.h>
 
 #include <optional>
+#include <tuple>
 
 #include "aotk.h"
 
@@ -337,112 +338,186 @@ void scaled_gemm(at::Tensor out, at::Tensor a, at::Tensor b, at::Tensor scale_a,
                op);
 }
 
+// ---- microscaled 4-bit ops and the sandwich norm -------------------------------
+//
+// These allocate their outputs and make every check here, with the error types
+// of the Python wrappers (ValueError; RuntimeError for tensors that are not on a
+// CUDA device), so that a wrapper is one call: for a decoded token the host's
+// time is most of a call's (12.5 -> 6.4 us for a small product).
+
+void check_on(const at::Tensor& t, const at::Tensor& first, const char* op, const char* name) {
+  check_cuda(t, op, name);
+  TORCH_CHECK_VALUE(t.device() == first.device(), "[", op, "] device mismatch: ", name, " is on ",
+                    t.device(), ", not on ", first.device());
+}
+
+int float_dtype(at::ScalarType t, const char* op) {
+  switch (t) {
+    case at::ScalarType::Float: return AOTK_FLOAT32;
+    case at::ScalarType::Half: return AOTK_FLOAT16;
+    case at::ScalarType::BFloat16: return AOTK_BFLOAT16;
+    default: break;
+  }
+  TORCH_CHECK_VALUE(false, "[", op, "] expects float32, float16 or bfloat16, got ", t);
+  return -1;
+}
+
 // Codes [rows, cols / 2] and scale tiles of a quantised matrix; returns cols.
-int64_t check_mxfp4(const at::Tensor& codes, const at::Tensor& scales, const char* op,
-                    const char* name) {
-  check_cuda(codes, op, name);
-  check_cuda(scales, op, "scales");
-  TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, "[", op, "] ",
-              name, " and its scales must be uint8");
-  TORCH_CHECK(codes.device() == scales.device(), "[", op, "] ", name,
-              " and its scales are not on the same device");
-  TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous(), "[", op, "] ", name,
-              " and its scales must be contiguous");
-  TORCH_CHECK(codes.dim() == 2 && codes.size(1) % 16 == 0, "[", op, "] ", name,
-              " must be [rows, cols / 2] with cols a multiple of 32, got ", codes.sizes());
+int64_t check_mxfp4(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& first,
+                    const char* op, const char* name) {
+  check_on(codes, first, op, name);
+  check_on(scales, first, op, "scales");
+  TORCH_CHECK_VALUE(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, "[", op,
+                    "] ", name, " and its scales must be uint8, got ", codes.scalar_type(), " and ",
+                    scales.scalar_type());
+  TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous(), "[", op, "] ", name,
+                    " and its scales must be contiguous");
+  TORCH_CHECK_VALUE(codes.dim() == 2 && codes.size(1) % 16 == 0, "[", op, "] ", name,
+                    " must be [rows, cols / 2] with cols a multiple of 32, got ", codes.sizes());
   const int64_t rows = codes.size(0), cols = 2 * codes.size(1);
-  TORCH_CHECK(scales.dim() == 3 && scales.size(0) == (rows + 127) / 128 &&
-                  scales.size(1) == (cols + 127) / 128 && scales.size(2) == 512,
-              "[", op, "] scales of ", name, " must be [", (rows + 127) / 128, ", ",
-              (cols + 127) / 128, ", 512], got ", scales.sizes());
+  TORCH_CHECK_VALUE(scales.dim() == 3 && scales.size(0) == (rows + 127) / 128 &&
+                        scales.size(1) == (cols + 127) / 128 && scales.size(2) == 512,
+                    "[", op, "] scales of ", name, " ", codes.sizes(), " must be [",
+                    (rows + 127) / 128, ", ", (cols + 127) / 128, ", 512], got ", scales.sizes());
   return cols;
 }
 
-void mxfp4_quantize(at::Tensor codes, at::Tensor scales, at::Tensor x) {
+std::tuple<at::Tensor, at::Tensor> mxfp4_quantize(const at::Tensor& x) {
   const char* op = "mxfp4_quantize";
   check_cuda(x, op, "x");
-  const int64_t cols = check_mxfp4(codes, scales, op, "codes");
-  TORCH_CHECK(codes.device() == x.device(), "[", op, "] x and codes are not on the same device");
-  TORCH_CHECK(x.dim() == 2 && x.size(0) == codes.size(0) && x.size(1) == cols, "[", op,
-              "] x must be [", codes.size(0), ", ", cols, "], got ", x.sizes());
-  const int64_t stride = row_stride(x, op, "x");
+  const int dtype = float_dtype(x.scalar_type(), op);
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) % 32 == 0, "[", op,
+                    "] x must be [rows, cols] with cols a multiple of 32, got ", x.sizes());
+  const int64_t rows = x.size(0), cols = x.size(1);
+  const bool dense = x.is_contiguous();
+  TORCH_CHECK_VALUE(dense || (x.stride(1) == 1 && x.stride(0) >= cols), "[", op,
+                    "] x must be contiguous or a 2-D view with contiguous rows");
   c10::cuda::CUDAGuard guard(x.device());
-  check_status(aotk_mxfp4_quantize(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), stride,
-                                   x.size(0), cols, aotk_dtype(x, op), current_stream(x)),
+  const auto bytes = x.options().dtype(at::kByte);
+  at::Tensor codes = at::empty({rows, cols / 2}, bytes);
+  at::Tensor scales = at::empty({(rows + 127) / 128, (cols + 127) / 128, 512}, bytes);
+  check_status(aotk_mxfp4_quantize(codes.data_ptr(), scales.data_ptr(), x.data_ptr(),
+                                   dense ? cols : x.stride(0), rows, cols, dtype,
+                                   current_stream(x)),
                op);
+  return {codes, scales};
 }
 
-void mxfp4_dequantize(at::Tensor out, at::Tensor codes, at::Tensor scales) {
+at::Tensor mxfp4_dequantize(const at::Tensor& codes, const at::Tensor& scales, at::ScalarType type) {
   const char* op = "mxfp4_dequantize";
-  check_cuda(out, op, "out");
-  const int64_t cols = check_mxfp4(codes, scales, op, "codes");
-  TORCH_CHECK(out.device() == codes.device(), "[", op, "] out and codes are not on the same device");
-  TORCH_CHECK(out.is_contiguous() && out.dim() == 2 && out.size(0) == codes.size(0) &&
-                  out.size(1) == cols,
-              "[", op, "] out must be a contiguous [", codes.size(0), ", ", cols, "], got ",
-              out.sizes());
-  c10::cuda::CUDAGuard guard(out.device());
+  const int64_t cols = check_mxfp4(codes, scales, codes, op, "codes");
+  const int dtype = float_dtype(type, op);
+  c10::cuda::CUDAGuard guard(codes.device());
+  at::Tensor out = at::empty({codes.size(0), cols}, codes.options().dtype(type));
   check_status(aotk_mxfp4_dequantize(out.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-                                     out.size(0), cols, aotk_dtype(out, op), current_stream(out)),
+                                     codes.size(0), cols, dtype, current_stream(codes)),
                op);
+  return out;
 }
 
-void mxfp4_gemm(at::Tensor out, at::Tensor a, at::Tensor a_scales, at::Tensor b,
-                at::Tensor b_scales) {
+// Checks the operands of a product and returns K.
+int64_t check_mxfp4_gemm(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b,
+                         const at::Tensor& b_scales, const char* op) {
+  const int64_t K = check_mxfp4(a, a_scales, a, op, "a");
+  const int64_t K2 = check_mxfp4(b, b_scales, a, op, "b");
+  TORCH_CHECK_VALUE(K == K2, "[", op, "] inner dims mismatch: ", K, " vs ", K2);
+  return K;
+}
+
+at::Tensor mxfp4_gemm(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b,
+                      const at::Tensor& b_scales, at::ScalarType out_dtype) {
   const char* op = "mxfp4_gemm";
-  check_cuda(out, op, "out");
-  const int64_t K = check_mxfp4(a, a_scales, op, "a");
-  TORCH_CHECK(check_mxfp4(b, b_scales, op, "b") == K, "[", op, "] inner dims mismatch: ", K,
-              " vs ", 2 * b.size(1));
-  TORCH_CHECK(out.device() == a.device() && b.device() == a.device(), "[", op,
-              "] tensors are not on one device");
-  TORCH_CHECK(out.is_contiguous() && out.dim() == 2 && out.size(0) == a.size(0) &&
-                  out.size(1) == b.size(0),
-              "[", op, "] out must be a contiguous [", a.size(0), ", ", b.size(0), "], got ",
-              out.sizes());
+  const int64_t K = check_mxfp4_gemm(a, a_scales, b, b_scales, op);
+  const int dtype = float_dtype(out_dtype, op);
+  c10::cuda::CUDAGuard guard(a.device());
+  at::Tensor out = at::empty({a.size(0), b.size(0)}, a.options().dtype(out_dtype));
+  check_status(aotk_mxfp4_gemm(out.data_ptr(), a.data_ptr(), a_scales.data_ptr(), b.data_ptr(),
+                               b_scales.data_ptr(), a.size(0), b.size(0), K, dtype,
+                               current_stream(a)),
+               op);
+  return out;
+}
+
+void mxfp4_gemm_out(at::Tensor out, const at::Tensor& a, const at::Tensor& a_scales,
+                    const at::Tensor& b, const at::Tensor& b_scales) {
+  const char* op = "mxfp4_gemm";
+  const int64_t K = check_mxfp4_gemm(a, a_scales, b, b_scales, op);
+  TORCH_CHECK_VALUE(out.device() == a.device() && out.is_contiguous() && out.dim() == 2 && out.size(0) == a.size(0) &&
+                        out.size(1) == b.size(0),
+                    "[", op, "] out must be a contiguous [", a.size(0), ", ", b.size(0), "] on ",
+                    a.device(), ", got ", out.sizes(), " on ", out.device());
+  const int dtype = float_dtype(out.scalar_type(), op);
   c10::cuda::CUDAGuard guard(a.device());
   check_status(aotk_mxfp4_gemm(out.data_ptr(), a.data_ptr(), a_scales.data_ptr(), b.data_ptr(),
-                               b_scales.data_ptr(), a.size(0), b.size(0), K, aotk_dtype(out, op),
+                               b_scales.data_ptr(), a.size(0), b.size(0), K, dtype,
                                current_stream(a)),
                op);
 }
 
-// gate: [gate_rows, cols] or [gate_rows, 1], row r of x using gate row
-// r / (rows / gate_rows).
-void sandwich_rmsnorm(at::Tensor out, at::Tensor h_out, at::Tensor x, at::Tensor residual,
-                      at::Tensor post_weight, at::Tensor pre_weight,
-                      std::optional<at::Tensor> gate, double residual_scale, double eps) {
+// gate broadcasts over x: last dim cols or 1, leading dims those of x from the
+// left and 1 after that.  Returns the number of its rows (each serves as many
+// consecutive rows of x).
+int64_t gate_rows(const at::Tensor& gate, const at::Tensor& x, const char* op) {
+  const int64_t missing = x.dim() - gate.dim();
+  TORCH_CHECK_VALUE(gate.dim() >= 1 && missing >= 0 &&
+                        (gate.size(-1) == x.size(-1) || gate.size(-1) == 1),
+                    "[", op, "] gate ", gate.sizes(), " does not broadcast over x ", x.sizes());
+  int64_t rows = 1;
+  bool ones = false;  // from here on only ones
+  for (int64_t i = 0; i < x.dim() - 1; ++i) {
+    const int64_t n = i < missing ? 1 : gate.size(i - missing);
+    if (!ones && n == x.size(i)) {
+      rows *= n;
+    } else {
+      ones = true;
+      TORCH_CHECK_VALUE(n == 1, "[", op, "] gate ", gate.sizes(), " must match leading dims of x ",
+                        x.sizes(), " and be 1 in the others");
+    }
+  }
+  return rows;
+}
+
+std::tuple<at::Tensor, at::Tensor> sandwich_rmsnorm(const at::Tensor& x, const at::Tensor& residual,
+                                                    const at::Tensor& post_weight,
+                                                    const at::Tensor& pre_weight,
+                                                    const std::optional<at::Tensor>& gate,
+                                                    double residual_scale, double eps) {
   const char* op = "sandwich_rmsnorm";
   check_cuda(x, op, "x");
-  check_same(x, residual, op, "x", "residual");
-  check_same(x, post_weight, op, "x", "post_weight");
-  check_same(x, pre_weight, op, "x", "pre_weight");
-  TORCH_CHECK(x.dim() >= 1 && x.sizes() == residual.sizes(), "[", op,
-              "] x and residual shapes differ: ", x.sizes(), " vs ", residual.sizes());
-  TORCH_CHECK(x.is_contiguous() && residual.is_contiguous() && post_weight.is_contiguous() &&
-                  pre_weight.is_contiguous(),
-              "[", op, "] inputs must be contiguous");
+  const int dtype = float_dtype(x.scalar_type(), op);
+  auto same = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.device() == x.device(), "[", op, "] device mismatch: ", name, " is on ",
+                      t.device(), ", x on ", x.device());
+    TORCH_CHECK_VALUE(t.scalar_type() == x.scalar_type(), "[", op, "] dtype mismatch: ", name, " ",
+                      t.scalar_type(), " vs x ", x.scalar_type());
+    TORCH_CHECK_VALUE(t.is_contiguous(), "[", op, "] ", name, " must be contiguous");
+  };
+  same(x, "x");
+  same(residual, "residual");
+  same(post_weight, "post_weight");
+  same(pre_weight, "pre_weight");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.sizes() == residual.sizes(), "[", op,
+                    "] shape mismatch: x ", x.sizes(), " vs residual ", residual.sizes());
   const int64_t cols = x.size(-1);
-  TORCH_CHECK(post_weight.dim() == 1 && pre_weight.dim() == 1 && post_weight.size(0) == cols &&
-                  pre_weight.size(0) == cols,
-              "[", op, "] weights must be [x.size(-1)]");
-  check_out_like(out, x, op);
-  check_out_like(h_out, x, op);
-  if (x.numel() == 0) return;
-  const int64_t rows = x.numel() / cols;
+  TORCH_CHECK_VALUE(post_weight.dim() == 1 && pre_weight.dim() == 1 &&
+                        post_weight.size(0) == cols && pre_weight.size(0) == cols,
+                    "[", op, "] weights must be [", cols, "], got ", post_weight.sizes(), " and ",
+                    pre_weight.sizes());
+  int64_t g_rows = 0;
   if (gate) {
-    check_same(x, *gate, op, "x", "gate");
-    TORCH_CHECK(gate->is_contiguous() && gate->dim() == 2, "[", op,
-                "] gate must be a contiguous [gate_rows, cols] or [gate_rows, 1]");
+    same(*gate, "gate");
+    g_rows = gate_rows(*gate, x, op);
   }
   c10::cuda::CUDAGuard guard(x.device());
-  check_status(aotk_sandwich_rmsnorm(out.data_ptr(), h_out.data_ptr(), x.data_ptr(),
-                                     residual.data_ptr(), post_weight.data_ptr(),
-                                     pre_weight.data_ptr(), gate ? gate->data_ptr() : nullptr,
-                                     gate ? gate->size(0) : 0, gate ? gate->size(1) : 0,
-                                     residual_scale, rows, cols, eps, aotk_dtype(x, op),
-                                     current_stream(x)),
-               op);
+  at::Tensor out = at::empty_like(x), h = at::empty_like(x);
+  if (x.numel() > 0)
+    check_status(aotk_sandwich_rmsnorm(out.data_ptr(), h.data_ptr(), x.data_ptr(),
+                                       residual.data_ptr(), post_weight.data_ptr(),
+                                       pre_weight.data_ptr(), gate ? gate->data_ptr() : nullptr,
+                                       g_rows, gate ? gate->size(-1) : 0, residual_scale,
+                                       x.numel() / cols, cols, eps, dtype, current_stream(x)),
+                 op);
+  return {out, h};
 }
 
 }  // namespace
@@ -485,20 +560,33 @@ TORCH_LIBRARY(aot_kernel, m) {
       "optimized) -> ()");
   m.impl("scaled_gemm", c10::kCUDA, &scaled_gemm);
 
-  m.def("mxfp4_quantize(Tensor! codes, Tensor! scales, Tensor x) -> ()");
+  m.def("mxfp4_quantize(Tensor x) -> (Tensor, Tensor)");
   m.impl("mxfp4_quantize", c10::kCUDA, &mxfp4_quantize);
 
-  m.def("mxfp4_dequantize(Tensor! out, Tensor codes, Tensor scales) -> ()");
+  m.def("mxfp4_dequantize(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
   m.impl("mxfp4_dequantize", c10::kCUDA, &mxfp4_dequantize);
 
   m.def(
-      "mxfp4_gemm(Tensor! out, Tensor a, Tensor a_scales, Tensor b, Tensor b_scales) -> ()");
+      "mxfp4_gemm(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, ScalarType out_dtype) -> "
+      "Tensor");
   m.impl("mxfp4_gemm", c10::kCUDA, &mxfp4_gemm);
 
   m.def(
-      "sandwich_rmsnorm(Tensor! out, Tensor! h_out, Tensor x, Tensor residual, Tensor post_weight, "
-      "Tensor pre_weight, Tensor? gate, float residual_scale, float eps) -> ()");
+      "mxfp4_gemm_out(Tensor! out, Tensor a, Tensor a_scales, Tensor b, Tensor b_scales) -> ()");
+  m.impl("mxfp4_gemm_out", c10::kCUDA, &mxfp4_gemm_out);
+
+  m.def(
+      "sandwich_rmsnorm(Tensor x, Tensor residual, Tensor post_weight, Tensor pre_weight, Tensor? "
+      "gate, float residual_scale, float eps) -> (Tensor, Tensor)");
   m.impl("sandwich_rmsnorm", c10::kCUDA, &sandwich_rmsnorm);
+}
+
+// Forward only, like the ops that write into `out`: outputs take no part in
+// autograd, whether or not a weight requires a gradient.
+TORCH_LIBRARY_IMPL(aot_kernel, AutogradCUDA, m) {
+  for (const char* name : {"mxfp4_quantize", "mxfp4_dequantize", "mxfp4_gemm", "mxfp4_gemm_out",
+                           "sandwich_rmsnorm"})
+    m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 // `import aot_kernel._C` runs the static registration above; the module itself is empty.

@@ -72,23 +72,6 @@ def test_wrappers_refuse_cpu_tensors():
         aot_kernel.sandwich_rmsnorm(torch.zeros(2, 8), torch.zeros(2, 8), w, w)
 
 
-@pytest.mark.parametrize("shape,rows", [((8,), 1), ((1, 1, 8), 1), ((2, 1, 8), 2), ((2, 1, 1), 2),
-                                        ((2, 3, 1), 6), ((2, 3, 8), 6), ((1,), 1)])
-def test_gate_rows(shape, rows):
-    from aot_kernel.norm import _gate_rows
-
-    g = _gate_rows(torch.zeros(shape), torch.zeros(2, 3, 8))
-    assert g.shape == (rows, shape[-1])
-
-
-@pytest.mark.parametrize("shape", [(), (3, 8), (1, 3, 8), (2, 3, 4), (4,), (1, 2, 3, 8), (3, 1)])
-def test_gate_refusals(shape):
-    from aot_kernel.norm import _gate_rows
-
-    with pytest.raises(ValueError):
-        _gate_rows(torch.zeros(shape), torch.zeros(2, 3, 8))
-
-
 BF16, F32, I8 = capi.BFLOAT16, capi.FLOAT32, capi.INT8
 
 

@@ -180,10 +180,33 @@ def test_refusals():
         with pytest.raises(ValueError):
             f(*args, **kw)
     for weights in ((w[:4], w), (w, w[:4]), (x, w)):
-        with pytest.raises(RuntimeError):
+        with pytest.raises(ValueError):
             f(x, x, *weights)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         f(x.double(), x.double(), w.double(), w.double())
+
+
+@pytest.mark.parametrize("shape", [(), (3, 8), (1, 3, 8), (2, 3, 4), (4,), (1, 2, 3, 8), (3, 1),
+                                   (3, 1, 8)])
+def test_gate_refusals(shape):
+    import torch
+
+    import aot_kernel
+
+    x, w = torch.zeros(2, 3, 8, device="cuda"), torch.ones(8, device="cuda")
+    with pytest.raises(ValueError):
+        aot_kernel.sandwich_rmsnorm(x, x, w, w, gate=torch.ones(shape, device="cuda"))
+
+
+def test_outputs_take_no_part_in_autograd():
+    import torch
+
+    import aot_kernel
+
+    x = torch.randn(4, 64, device="cuda")
+    w = torch.nn.Parameter(torch.ones(64, device="cuda"))
+    out, h = aot_kernel.sandwich_rmsnorm(x, x, w, w, gate=w)
+    assert not out.requires_grad and not h.requires_grad
 
 
 def test_stream_and_graph():
