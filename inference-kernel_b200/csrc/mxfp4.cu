@@ -19,132 +19,170 @@
 // to no row or block are written as 0.
 //
 // Both kernels are bound by HBM.  A half-warp owns one 128-column tile of one
-// row (a lane 8 elements: one or two 16-byte loads, one 4-byte word of codes;
-// four lanes a block, one shuffle pair for its maximum; 16 lanes one 4-byte
-// word of scales), and each lane has kUnroll such loads in flight.
+// row: a lane 8 elements (one 16-byte or 32-byte load), which make one 4-byte word
+// of codes; four lanes a block, two shuffles for its maximum; 16 lanes one 4-byte
+// word of scales, two more.  Each lane has kUnroll loads in flight.
 #include "common.h"
 #include "mxfp4.cuh"
+#include "sm100.cuh"
 #include "vec.cuh"
 
 namespace aotk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;                              // tiles in flight per half-warp
-constexpr int kTilesPerBlock = kThreads / 16 * kUnroll;  // 128-column row tiles
+constexpr int kRowTiles = kThreads / 16;  // 128-column row tiles per block at a time
+constexpr int kUnroll = 4;                // of each half-warp, kRowTiles apart
 
-// Eight consecutive elements as 16-byte vectors (kVec) or one by one.
-template <typename T, bool kVec>
+// Row tile t of the problem is columns [128 (t % tiles_k), +128) of row t / tiles_k.
+// A block's tiles are consecutive; step = kRowTiles tiles on.
+struct Walk {
+  int tiles_k;
+  int step_rows, step_tiles;  // kRowTiles / tiles_k and the remainder
+};
+
+// This half-warp's first tile: one division by a uniform value and one of small
+// numbers per thread, and none from tile to tile.
+__device__ __forceinline__ void first_tile(const Walk& w, int64_t& row, int& kt) {
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowTiles * kUnroll);
+  const int64_t row0 = t / w.tiles_k;
+  const unsigned in_row = static_cast<unsigned>(t - row0 * w.tiles_k) + threadIdx.x / 16;
+  const unsigned more = in_row / static_cast<unsigned>(w.tiles_k);
+  row = row0 + more;
+  kt = static_cast<int>(in_row - more * w.tiles_k);
+}
+
+__device__ __forceinline__ void next_tile(const Walk& w, int64_t& row, int& kt) {
+  row += w.step_rows;
+  kt += w.step_tiles;
+  if (kt >= w.tiles_k) {
+    kt -= w.tiles_k;
+    ++row;
+  }
+}
+
+__device__ __forceinline__ int64_t scale_word(int64_t row, int kt, int tiles_k) {
+  const int r = static_cast<int>(row & 127);
+  return ((row >> 7) * tiles_k + kt) * 512 + (r & 31) * 16 + (r >> 5) * 4;
+}
+
+enum : int { kElements = 0, kVectors = 1, kWide = 2 };  // accesses of 1, 16 / sizeof, 32 / sizeof
+
+// Eight consecutive elements of a lane.
+template <typename T, int kAccess>
 struct Eight {
-  static constexpr int kWords = 8 / Elem<T>::kPerVec;
+  static constexpr int kWords = sizeof(T) / 2;  // 16-byte vectors
   uint4 raw[kWords];
-  T one[kVec ? 1 : 8];
 
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (!kVec) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) one[i] = Elem<T>::from_f(0.f);
-    }
   }
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kVec) {
+    if constexpr (kAccess == kWide) {
+      ld_stream32(p, raw[0], raw[1]);
+    } else if constexpr (kAccess == kVectors) {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) raw[i] = ld_stream(reinterpret_cast<const uint4*>(p) + i);
     } else {
+      T* e = reinterpret_cast<T*>(raw);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) one[i] = p[i];
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
     }
   }
   __device__ __forceinline__ void get(float* f) const {
-    if constexpr (kVec) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) Elem<T>::unpack(raw[i], f + i * Elem<T>::kPerVec);
+    for (int i = 0; i < kWords; ++i) Elem<T>::unpack(raw[i], f + i * Elem<T>::kPerVec);
+  }
+  // Bits of the largest magnitude as fp32.  Magnitudes order like their bits,
+  // with infinity above all numbers and NaN above it; 16-bit ones are compared
+  // in pairs.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+        m = max(m, max(max(raw[i].x & 0x7FFFFFFFu, raw[i].y & 0x7FFFFFFFu),
+                       max(raw[i].z & 0x7FFFFFFFu, raw[i].w & 0x7FFFFFFFu)));
+      return m;
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f(one[i]);
+      const uint32_t m = __vmaxu2(__vmaxu2(raw[0].x & 0x7FFF7FFFu, raw[0].y & 0x7FFF7FFFu),
+                                  __vmaxu2(raw[0].z & 0x7FFF7FFFu, raw[0].w & 0x7FFF7FFFu));
+      const uint16_t h = static_cast<uint16_t>(max(m & 0xFFFFu, m >> 16));
+      return __float_as_uint(Elem<T>::to_f(*reinterpret_cast<const T*>(&h)));
     }
   }
 };
 
-// Row tile t of the padded problem: row t / tiles_k, columns [128 (t % tiles_k), +128).
-template <typename T, bool kVec>
+template <typename T, int kAccess>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                    const T* __restrict__ x, int64_t stride, int64_t rows, int64_t cols,
-                    int tiles_k, int64_t tiles) {
+                    const T* __restrict__ x, int64_t stride, int64_t rows, int64_t rows_padded,
+                    int cols, const Walk walk) {
   const int lane16 = threadIdx.x & 15;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kTilesPerBlock + threadIdx.x / 16;
-  Eight<T, kVec> in[kUnroll];
-  int64_t row[kUnroll], col[kUnroll];
+  sm100::pdl_launch_dependents();
+  sm100::pdl_wait_prior();
+  Eight<T, kAccess> in[kUnroll];
+  int64_t row[kUnroll];
+  int kt[kUnroll];
+  first_tile(walk, row[0], kt[0]);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t t = t0 + u * (kThreads / 16);
-    row[u] = t / tiles_k;
-    col[u] = (t - row[u] * tiles_k) * 128 + lane16 * 8;
-    if (row[u] < rows && col[u] < cols)
-      in[u].load(x + row[u] * stride + col[u]);
+    if (u > 0) {
+      row[u] = row[u - 1];
+      kt[u] = kt[u - 1];
+      next_tile(walk, row[u], kt[u]);
+    }
+    const int col = kt[u] * 128 + lane16 * 8;
+    if (row[u] < rows && col < cols)
+      in[u].load(x + row[u] * stride + col);
     else
       in[u].zero();
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    float f[8];
-    in[u].get(f);
-    // Magnitudes as integers: they order like the values, and a NaN is above
-    // an infinity, which is above all else.
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+    uint32_t top = in[u].top();
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t biased = top >> 23;
-    const uint32_t byte = biased == 255 ? 255u : biased > 2 ? biased - 2 : 0u;
-    const float inv = __uint_as_float((254u - (byte == 255 ? 254u : byte)) << 23);
+    const bool bad = biased == 255;
+    const uint32_t byte = bad ? 255u : biased > 2 ? biased - 2 : 0u;
+    float f[8];
+    in[u].get(f);
+    const float inv = __uint_as_float((254u - (bad ? 0u : byte)) << 23);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] *= inv;
-    uint32_t word = mx::encode_e2m1x8(f);
-    if (byte == 255) word = 0;
-    const int base = threadIdx.x & 16;
-    const uint32_t b0 = __shfl_sync(0xffffffffu, byte, base);
-    const uint32_t b1 = __shfl_sync(0xffffffffu, byte, base + 4);
-    const uint32_t b2 = __shfl_sync(0xffffffffu, byte, base + 8);
-    const uint32_t b3 = __shfl_sync(0xffffffffu, byte, base + 12);
-    const int64_t t = t0 + u * (kThreads / 16);
-    if (t < tiles) {
-      if (row[u] < rows && col[u] < cols)
-        *reinterpret_cast<uint32_t*>(codes + (row[u] * cols + col[u]) / 2) = word;
-      if (lane16 == 0) {
-        const int64_t tile = (row[u] / 128) * tiles_k + (t - row[u] * tiles_k);
-        const int r = static_cast<int>(row[u] % 128);
-        *reinterpret_cast<uint32_t*>(scales + tile * 512 + (r % 32) * 16 + r / 32 * 4) =
-            b0 | b1 << 8 | b2 << 16 | b3 << 24;
-      }
-    }
+    const uint32_t word = bad ? 0u : mx::encode_e2m1x8(f);
+    uint32_t four = byte << (lane16 / 4 * 8);
+    four |= __shfl_xor_sync(0xffffffffu, four, 4);
+    four |= __shfl_xor_sync(0xffffffffu, four, 8);
+    const int col = kt[u] * 128 + lane16 * 8;
+    if (row[u] < rows && col < cols)
+      *reinterpret_cast<uint32_t*>(codes + row[u] * (cols / 2) + col / 2) = word;
+    if (lane16 == 0 && row[u] < rows_padded)
+      *reinterpret_cast<uint32_t*>(scales + scale_word(row[u], kt[u], walk.tiles_k)) = four;
   }
 }
 
-template <typename T, bool kVec>
+template <typename T, int kAccess>
 __global__ void __launch_bounds__(kThreads)
     dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes,
-                      const uint8_t* __restrict__ scales, int64_t rows, int64_t cols, int tiles_k,
-                      int64_t tiles) {
+                      const uint8_t* __restrict__ scales, int64_t rows, int cols, const Walk walk) {
   const int lane16 = threadIdx.x & 15;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kTilesPerBlock + threadIdx.x / 16;
+  sm100::pdl_launch_dependents();
+  sm100::pdl_wait_prior();
   uint32_t word[kUnroll], byte[kUnroll];
-  int64_t at[kUnroll];
+  int64_t at[kUnroll], row;
+  int kt;
+  first_tile(walk, row, kt);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t t = t0 + u * (kThreads / 16);
-    const int64_t row = t / tiles_k;
-    const int64_t kt = t - row * tiles_k;
-    const int64_t col = kt * 128 + lane16 * 8;
-    at[u] = t < tiles && col < cols ? row * cols + col : -1;
+    if (u > 0) next_tile(walk, row, kt);
+    const int col = kt * 128 + lane16 * 8;
+    at[u] = row < rows && col < cols ? row * cols + col : -1;
     if (at[u] >= 0) {
       word[u] = *reinterpret_cast<const uint32_t*>(codes + at[u] / 2);
-      const int r = static_cast<int>(row % 128);
-      byte[u] = scales[((row / 128) * tiles_k + kt) * 512 + (r % 32) * 16 + r / 32 * 4 + lane16 / 4];
+      byte[u] = scales[scale_word(row, kt, walk.tiles_k) + lane16 / 4];
     }
   }
 #pragma unroll
@@ -155,14 +193,16 @@ __global__ void __launch_bounds__(kThreads)
     const float s = mx::scale_value(byte[u]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] *= s;
-    if constexpr (kVec) {
+    T* o = out + at[u];
+    if constexpr (kAccess == kWide) {
+      st_stream32(o, Elem<T>::pack(f), Elem<T>::pack(f + 4));
+    } else if constexpr (kAccess == kVectors) {
 #pragma unroll
       for (int i = 0; i < 8 / Elem<T>::kPerVec; ++i)
-        st_stream(reinterpret_cast<uint4*>(out + at[u]) + i,
-                  Elem<T>::pack(f + i * Elem<T>::kPerVec));
+        st_stream(reinterpret_cast<uint4*>(o) + i, Elem<T>::pack(f + i * Elem<T>::kPerVec));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[at[u] + i] = Elem<T>::from_f(f[i]);
+      for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_f(f[i]);
     }
   }
 }
@@ -184,46 +224,69 @@ int check(const char* who, const void* values, const void* codes, const void* sc
   return AOTK_OK;
 }
 
-int blocks_for(const char* who, int64_t tiles, unsigned* blocks) {
-  const int64_t n = (tiles + kTilesPerBlock - 1) / kTilesPerBlock;
+template <typename... P, typename... A>
+int launch(const char* who, void (*kernel)(P...), int64_t row_tiles, cudaStream_t s, A... args) {
+  const int64_t n = (row_tiles + kRowTiles * kUnroll - 1) / (kRowTiles * kUnroll);
   if (n > 0x7fffffffLL) return fail(AOTK_ERR_UNSUPPORTED, "%s: too many elements", who);
-  *blocks = static_cast<unsigned>(n);
-  return AOTK_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(n), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(AOTK_ERR_CUDA, "%s launch: %s", who, cudaGetErrorString(e));
+  return check_launch(who);
+}
+
+Walk walk_of(int64_t cols) {
+  const int tiles_k = static_cast<int>((cols + 127) / 128);
+  return Walk{tiles_k, kRowTiles / tiles_k, kRowTiles % tiles_k};
+}
+
+// Rows of 32 columns are 64 or 128 bytes, so the base and the row stride decide.
+template <typename T>
+int access_of(const void* p, int64_t stride) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * sizeof(T));
+  if (sizeof(T) == 4 && bits % 32 == 0) return kWide;
+  return bits % 16 == 0 ? kVectors : kElements;
 }
 
 template <typename T>
 int quantize(void* codes, void* scales, const void* x, int64_t stride, int64_t rows, int64_t cols,
              cudaStream_t s) {
-  const int tiles_k = static_cast<int>((cols + 127) / 128);
-  const int64_t tiles = (rows + 127) / 128 * 128 * tiles_k;
-  unsigned blocks;
-  if (int st = blocks_for("aotk_mxfp4_quantize", tiles, &blocks)) return st;
-  const bool vec = aligned16(x) && stride * static_cast<int64_t>(sizeof(T)) % 16 == 0;
-  auto* c = static_cast<uint8_t*>(codes);
-  auto* sc = static_cast<uint8_t*>(scales);
-  auto* xt = static_cast<const T*>(x);
-  if (vec)
-    quantize_kernel<T, true><<<blocks, kThreads, 0, s>>>(c, sc, xt, stride, rows, cols, tiles_k, tiles);
-  else
-    quantize_kernel<T, false><<<blocks, kThreads, 0, s>>>(c, sc, xt, stride, rows, cols, tiles_k, tiles);
-  return check_launch("aotk_mxfp4_quantize");
+  const char* who = "aotk_mxfp4_quantize";
+  const Walk walk = walk_of(cols);
+  const int64_t padded = (rows + 127) / 128 * 128;
+  auto run = [&](auto kernel) {
+    return launch(who, kernel, padded * walk.tiles_k, s, static_cast<uint8_t*>(codes),
+                  static_cast<uint8_t*>(scales), static_cast<const T*>(x), stride, rows, padded,
+                  static_cast<int>(cols), walk);
+  };
+  const int access = access_of<T>(x, rows > 1 ? stride : 0);
+  if constexpr (sizeof(T) == 4)
+    if (access == kWide) return run(quantize_kernel<T, kWide>);
+  return access == kVectors ? run(quantize_kernel<T, kVectors>) : run(quantize_kernel<T, kElements>);
 }
 
 template <typename T>
 int dequantize(void* out, const void* codes, const void* scales, int64_t rows, int64_t cols,
                cudaStream_t s) {
-  const int tiles_k = static_cast<int>((cols + 127) / 128);
-  const int64_t tiles = rows * tiles_k;
-  unsigned blocks;
-  if (int st = blocks_for("aotk_mxfp4_dequantize", tiles, &blocks)) return st;
-  auto* o = static_cast<T*>(out);
-  auto* c = static_cast<const uint8_t*>(codes);
-  auto* sc = static_cast<const uint8_t*>(scales);
-  if (aligned16(out))
-    dequantize_kernel<T, true><<<blocks, kThreads, 0, s>>>(o, c, sc, rows, cols, tiles_k, tiles);
-  else
-    dequantize_kernel<T, false><<<blocks, kThreads, 0, s>>>(o, c, sc, rows, cols, tiles_k, tiles);
-  return check_launch("aotk_mxfp4_dequantize");
+  const char* who = "aotk_mxfp4_dequantize";
+  const Walk walk = walk_of(cols);
+  auto run = [&](auto kernel) {
+    return launch(who, kernel, rows * walk.tiles_k, s, static_cast<T*>(out),
+                  static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows,
+                  static_cast<int>(cols), walk);
+  };
+  const int access = access_of<T>(out, 0);
+  if constexpr (sizeof(T) == 4)
+    if (access == kWide) return run(dequantize_kernel<T, kWide>);
+  return access == kVectors ? run(dequantize_kernel<T, kVectors>)
+                            : run(dequantize_kernel<T, kElements>);
 }
 
 }  // namespace

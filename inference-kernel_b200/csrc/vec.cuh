@@ -21,6 +21,24 @@ __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
 // 16-byte load through L1 (for data reused by several warps, e.g. norm weights).
 __device__ __forceinline__ uint4 ld_cached(const uint4* p) { return __ldg(p); }
 
+// Read-only 32-byte load (32-byte aligned) that bypasses L1 allocation: a lane's
+// two vectors as one request, where two 16-byte loads would fetch each 32-byte
+// sector twice.
+__device__ __forceinline__ void ld_stream32(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z),
+                 "=r"(b.w)
+               : "l"(p));
+}
+
+__device__ __forceinline__ void st_stream32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               :
+               : "l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z),
+                 "r"(b.w)
+               : "memory");
+}
+
 __device__ __forceinline__ void st_stream(uint4* p, const uint4& v) {
   asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1, %2, %3, %4};"
                :
