@@ -18,10 +18,15 @@
 // which the tensor cores' scale loads take them.  Bytes of a tile that belong
 // to no row or block are written as 0.
 //
-// Both kernels are bound by HBM.  A half-warp owns one 128-column tile of one
-// row: a lane 8 elements (one 16-byte or 32-byte load), which make one 4-byte word
-// of codes; four lanes a block, two shuffles for its maximum; 16 lanes one 4-byte
-// word of scales, two more.  Each lane has kUnroll loads in flight.
+// Both kernels stream HBM, and what has to be kept down for that is the
+// arithmetic per element: a lane owns whole blocks of 32 elements, so that the
+// index arithmetic, the maximum and the scale are paid once per block and no lane
+// waits for another, apart from two shuffles that make one 4-byte word of the
+// scales of four neighbours.  (With four lanes to a block the quantiser issued
+// 132 instructions per 8 elements and ran at 0.58 of the copy rate.)  A lane's 64
+// or 128 bytes move as 32-byte accesses, whole sectors each.
+#include <type_traits>
+
 #include "common.h"
 #include "mxfp4.cuh"
 #include "sm100.cuh"
@@ -31,178 +36,248 @@ namespace aotk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowTiles = kThreads / 16;  // 128-column row tiles per block at a time
-constexpr int kUnroll = 4;                // of each half-warp, kRowTiles apart
+constexpr int kLanes = kThreads;  // blocks of 32 per thread block and step
 
-// Row tile t of the problem is columns [128 (t % tiles_k), +128) of row t / tiles_k.
-// A block's tiles are consecutive; step = kRowTiles tiles on.
+// Item t of the padded problem is item t % items_k of row t / items_k; a thread's
+// items are kLanes apart.
 struct Walk {
-  int tiles_k;
-  int step_rows, step_tiles;  // kRowTiles / tiles_k and the remainder
+  int items_k;
+  int step_rows, step_items;  // kLanes / items_k and the remainder
 };
 
-// This half-warp's first tile: one division by a uniform value and one of small
-// numbers per thread, and none from tile to tile.
-__device__ __forceinline__ void first_tile(const Walk& w, int64_t& row, int& kt) {
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowTiles * kUnroll);
-  const int64_t row0 = t / w.tiles_k;
-  const unsigned in_row = static_cast<unsigned>(t - row0 * w.tiles_k) + threadIdx.x / 16;
-  const unsigned more = in_row / static_cast<unsigned>(w.tiles_k);
+// This thread's first item: one division by a uniform value and one of small
+// numbers, and none from item to item.
+template <int U>
+__device__ __forceinline__ void first_item(const Walk& w, int64_t& row, int& kb) {
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kLanes * U);
+  const int64_t row0 = t / w.items_k;
+  const unsigned in_row = static_cast<unsigned>(t - row0 * w.items_k) + threadIdx.x;
+  const unsigned more = in_row / static_cast<unsigned>(w.items_k);
   row = row0 + more;
-  kt = static_cast<int>(in_row - more * w.tiles_k);
+  kb = static_cast<int>(in_row - more * w.items_k);
 }
 
-__device__ __forceinline__ void next_tile(const Walk& w, int64_t& row, int& kt) {
+__device__ __forceinline__ void next_item(const Walk& w, int64_t& row, int& kb) {
   row += w.step_rows;
-  kt += w.step_tiles;
-  if (kt >= w.tiles_k) {
-    kt -= w.tiles_k;
+  kb += w.step_items;
+  if (kb >= w.items_k) {
+    kb -= w.items_k;
     ++row;
   }
 }
 
-__device__ __forceinline__ int64_t scale_word(int64_t row, int kt, int tiles_k) {
+// Offset of the scale byte of block kb of a row.
+__device__ __forceinline__ int64_t scale_byte(int64_t row, int kb, int blocks_k) {
   const int r = static_cast<int>(row & 127);
-  return ((row >> 7) * tiles_k + kt) * 512 + (r & 31) * 16 + (r >> 5) * 4;
+  return ((row >> 7) * (blocks_k >> 2) + (kb >> 2)) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (kb & 3);
 }
 
-enum : int { kElements = 0, kVectors = 1, kWide = 2 };  // accesses of 1, 16 / sizeof, 32 / sizeof
+// The larger magnitude of each pair, NaN if either is; the sign is of no use.
+template <typename T>
+__device__ __forceinline__ uint32_t max_abs(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (sizeof(T) == 4)
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else if constexpr (std::is_same_v<T, __half>)
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
-// Eight consecutive elements of a lane.
-template <typename T, int kAccess>
-struct Eight {
-  static constexpr int kWords = sizeof(T) / 2;  // 16-byte vectors
-  uint4 raw[kWords];
+// One block of 32 elements in registers.
+template <typename T>
+struct Block {
+  static constexpr int kWords = 8 * sizeof(T);  // 32-bit words
+  uint32_t w[kWords];
 
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
   }
+  // p aligned to 32 bytes
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kAccess == kWide) {
-      ld_stream32(p, raw[0], raw[1]);
-    } else if constexpr (kAccess == kVectors) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) raw[i] = ld_stream(reinterpret_cast<const uint4*>(p) + i);
-    } else {
-      T* e = reinterpret_cast<T*>(raw);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = p[i];
+    for (int i = 0; i < kWords; i += 8) {
+      uint4 a, b;
+      ld_stream32(reinterpret_cast<const uint32_t*>(p) + i, a, b);
+      w[i] = a.x, w[i + 1] = a.y, w[i + 2] = a.z, w[i + 3] = a.w;
+      w[i + 4] = b.x, w[i + 5] = b.y, w[i + 6] = b.z, w[i + 7] = b.w;
     }
   }
-  __device__ __forceinline__ void get(float* f) const {
+  // Any p: the aligned 16-byte vectors around the block, through L1 since
+  // neighbours share them, shifted into place - or, where such a vector would
+  // reach out of [begin, end), element by element.
+  __device__ __forceinline__ void load_any(const T* p, const T* begin, const T* end) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uintptr_t lo = at & ~static_cast<uintptr_t>(15);
+    const uintptr_t hi = lo + (kWords * 4 + 16);
+    if (lo >= reinterpret_cast<uintptr_t>(begin) && hi <= reinterpret_cast<uintptr_t>(end)) {
+      const uint4* v = reinterpret_cast<const uint4*>(lo);
+      uint32_t r[kWords + 4];
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) Elem<T>::unpack(raw[i], f + i * Elem<T>::kPerVec);
-  }
-  // Bits of the largest magnitude as fp32.  Magnitudes order like their bits,
-  // with infinity above all numbers and NaN above it; 16-bit ones are compared
-  // in pairs.
-  __device__ __forceinline__ uint32_t top() const {
-    if constexpr (sizeof(T) == 4) {
-      uint32_t m = 0;
+      for (int i = 0; i < kWords / 4 + 1; ++i) {
+        const uint4 q = ld_cached(v + i);
+        r[4 * i] = q.x, r[4 * i + 1] = q.y, r[4 * i + 2] = q.z, r[4 * i + 3] = q.w;
+      }
+      const bool two = at & 8, one = at & 4;
 #pragma unroll
-      for (int i = 0; i < kWords; ++i)
-        m = max(m, max(max(raw[i].x & 0x7FFFFFFFu, raw[i].y & 0x7FFFFFFFu),
-                       max(raw[i].z & 0x7FFFFFFFu, raw[i].w & 0x7FFFFFFFu)));
-      return m;
+      for (int i = 0; i < kWords + 2; ++i) r[i] = two ? r[i + 2] : r[i];
+#pragma unroll
+      for (int i = 0; i < kWords + 1; ++i) r[i] = one ? r[i + 1] : r[i];
+      const uint32_t bits = (at & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(r[i], r[i + 1], bits);
     } else {
-      const uint32_t m = __vmaxu2(__vmaxu2(raw[0].x & 0x7FFF7FFFu, raw[0].y & 0x7FFF7FFFu),
-                                  __vmaxu2(raw[0].z & 0x7FFF7FFFu, raw[0].w & 0x7FFF7FFFu));
-      const uint16_t h = static_cast<uint16_t>(max(m & 0xFFFFu, m >> 16));
-      return __float_as_uint(Elem<T>::to_f(*reinterpret_cast<const T*>(&h)));
+      T e[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) e[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (sizeof(T) == 4)
+          w[i] = __float_as_uint(e[i]);
+        else
+          w[i] = Elem<T>::pack2(Elem<T>::to_f(e[2 * i]), Elem<T>::to_f(e[2 * i + 1]));
+      }
+    }
+  }
+  // Exponent field of the largest magnitude as fp32: 255 for a NaN or an infinity.
+  __device__ __forceinline__ uint32_t top_exponent() const {
+    uint32_t m = w[0];
+#pragma unroll
+    for (int i = 1; i < kWords; ++i) m = max_abs<T>(m, w[i]);
+    if constexpr (sizeof(T) == 4) {
+      return (m >> 23) & 255u;
+    } else {
+      m = max_abs<T>(m, m >> 16 | m << 16);
+      const uint16_t h = static_cast<uint16_t>(m);
+      return (__float_as_uint(Elem<T>::to_f(*reinterpret_cast<const T*>(&h))) >> 23) & 255u;
+    }
+  }
+  // Elements [8 i, 8 i + 8)
+  __device__ __forceinline__ void get8(int i, float* f) const {
+    constexpr int n = 2 * sizeof(T);
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        f[j] = __uint_as_float(w[n * i + j]);
+      } else {
+        const float2 t = Elem<T>::unpack2(w[n * i + j]);
+        f[2 * j] = t.x;
+        f[2 * j + 1] = t.y;
+      }
     }
   }
 };
 
-template <typename T, int kAccess>
+// Items (blocks) per thread when quantising: 128 bytes in flight.
+template <typename T>
+constexpr int kItems = 4 / sizeof(T);
+
+template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                     const T* __restrict__ x, int64_t stride, int64_t rows, int64_t rows_padded,
                     int cols, const Walk walk) {
-  const int lane16 = threadIdx.x & 15;
+  constexpr int U = kItems<T>;
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
-  Eight<T, kAccess> in[kUnroll];
-  int64_t row[kUnroll];
-  int kt[kUnroll];
-  first_tile(walk, row[0], kt[0]);
+  Block<T> in[U];
+  int64_t row[U];
+  int kb[U];
+  first_item<U>(walk, row[0], kb[0]);
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     if (u > 0) {
       row[u] = row[u - 1];
-      kt[u] = kt[u - 1];
-      next_tile(walk, row[u], kt[u]);
+      kb[u] = kb[u - 1];
+      next_item(walk, row[u], kb[u]);
     }
-    const int col = kt[u] * 128 + lane16 * 8;
-    if (row[u] < rows && col < cols)
-      in[u].load(x + row[u] * stride + col);
-    else
+    if (row[u] < rows && kb[u] * 32 < cols) {
+      const T* p = x + row[u] * stride + kb[u] * 32;
+      if constexpr (kAligned)
+        in[u].load(p);
+      else
+        in[u].load_any(p, x, x + (rows - 1) * stride + cols);
+    } else {
       in[u].zero();
+    }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    uint32_t top = in[u].top();
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t biased = top >> 23;
-    const bool bad = biased == 255;
-    const uint32_t byte = bad ? 255u : biased > 2 ? biased - 2 : 0u;
-    float f[8];
-    in[u].get(f);
+  for (int u = 0; u < U; ++u) {
+    const uint32_t e = in[u].top_exponent();
+    const bool bad = e == 255;
+    const uint32_t byte = bad ? 255u : e > 2 ? e - 2 : 0u;
     const float inv = __uint_as_float((254u - (bad ? 0u : byte)) << 23);
+    uint32_t word[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= inv;
-    const uint32_t word = bad ? 0u : mx::encode_e2m1x8(f);
-    uint32_t four = byte << (lane16 / 4 * 8);
-    four |= __shfl_xor_sync(0xffffffffu, four, 4);
-    four |= __shfl_xor_sync(0xffffffffu, four, 8);
-    const int col = kt[u] * 128 + lane16 * 8;
-    if (row[u] < rows && col < cols)
-      *reinterpret_cast<uint32_t*>(codes + row[u] * (cols / 2) + col / 2) = word;
-    if (lane16 == 0 && row[u] < rows_padded)
-      *reinterpret_cast<uint32_t*>(scales + scale_word(row[u], kt[u], walk.tiles_k)) = four;
+    for (int i = 0; i < 4; ++i) {
+      float f[8];
+      in[u].get8(i, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= inv;
+      word[i] = bad ? 0u : mx::encode_e2m1x8(f);
+    }
+    // Four neighbours are a row's four blocks of one scale tile.
+    uint32_t four = byte << ((threadIdx.x & 3) * 8);
+    four |= __shfl_xor_sync(0xffffffffu, four, 1);
+    four |= __shfl_xor_sync(0xffffffffu, four, 2);
+    if (row[u] < rows && kb[u] * 32 < cols)
+      *reinterpret_cast<uint4*>(codes + row[u] * (cols / 2) + kb[u] * 16) =
+          make_uint4(word[0], word[1], word[2], word[3]);
+    if ((threadIdx.x & 3) == 0 && row[u] < rows_padded)
+      *reinterpret_cast<uint32_t*>(scales + scale_byte(row[u], kb[u], walk.items_k)) = four;
   }
 }
 
-template <typename T, int kAccess>
+// Elements per item when reading back: 32 bytes of output, so that a warp's
+// stores are one run (whole blocks per lane gave 42.4 -> 46.8 us for 14336 x 4096
+// fp32, and too few threads where there is little to do).
+template <typename T>
+constexpr int kOutItem = 32 / sizeof(T);
+constexpr int kOutUnroll = 4;
+
+template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
     dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes,
                       const uint8_t* __restrict__ scales, int64_t rows, int cols, const Walk walk) {
-  const int lane16 = threadIdx.x & 15;
+  constexpr int E = kOutItem<T>, U = kOutUnroll;
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
-  uint32_t word[kUnroll], byte[kUnroll];
-  int64_t at[kUnroll], row;
-  int kt;
-  first_tile(walk, row, kt);
+  uint32_t word[U][E / 8], byte[U];
+  int64_t at[U], row;
+  int item;
+  first_item<U>(walk, row, item);
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    if (u > 0) next_tile(walk, row, kt);
-    const int col = kt * 128 + lane16 * 8;
+  for (int u = 0; u < U; ++u) {
+    if (u > 0) next_item(walk, row, item);
+    const int col = item * E;
     at[u] = row < rows && col < cols ? row * cols + col : -1;
     if (at[u] >= 0) {
-      word[u] = *reinterpret_cast<const uint32_t*>(codes + at[u] / 2);
-      byte[u] = scales[scale_word(row, kt, walk.tiles_k) + lane16 / 4];
+      if constexpr (E == 16) {
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + at[u] / 2);
+        word[u][0] = w.x;
+        word[u][1] = w.y;
+      } else {
+        word[u][0] = *reinterpret_cast<const uint32_t*>(codes + at[u] / 2);
+      }
+      byte[u] = scales[scale_byte(row, col / 32, walk.items_k / (32 / E))];
     }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     if (at[u] < 0) continue;
-    float f[8];
-    mx::decode_e2m1x8(word[u], f);
+    float f[E];
+#pragma unroll
+    for (int j = 0; j < E; j += 8) mx::decode_e2m1x8(word[u][j / 8], f + j);
     const float s = mx::scale_value(byte[u]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= s;
-    T* o = out + at[u];
-    if constexpr (kAccess == kWide) {
-      st_stream32(o, Elem<T>::pack(f), Elem<T>::pack(f + 4));
-    } else if constexpr (kAccess == kVectors) {
-#pragma unroll
-      for (int i = 0; i < 8 / Elem<T>::kPerVec; ++i)
-        st_stream(reinterpret_cast<uint4*>(o) + i, Elem<T>::pack(f + i * Elem<T>::kPerVec));
+    for (int j = 0; j < E; ++j) f[j] *= s;
+    if constexpr (kAligned) {
+      st_stream32(out + at[u], Elem<T>::pack(f), Elem<T>::pack(f + E / 2));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = Elem<T>::from_f(f[i]);
+      for (int j = 0; j < E; ++j) out[at[u] + j] = Elem<T>::from_f(f[j]);
     }
   }
 }
@@ -219,14 +294,16 @@ int check(const char* who, const void* values, const void* codes, const void* sc
     return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   if (!aligned16(codes) || !aligned16(scales))
     return fail(AOTK_ERR_UNSUPPORTED, "%s: codes and scales must be 16-byte aligned", who);
-  if (cols > 0x7fffffffLL || rows > 0x7fffffffLL)
-    return fail(AOTK_ERR_UNSUPPORTED, "%s: extents above 2^31 - 1", who);
+  if (cols > 0x7fffff00LL || rows > 0x7fffff00LL)
+    return fail(AOTK_ERR_UNSUPPORTED, "%s: extents above 2^31 - 256", who);
   return AOTK_OK;
 }
 
 template <typename... P, typename... A>
-int launch(const char* who, void (*kernel)(P...), int64_t row_tiles, cudaStream_t s, A... args) {
-  const int64_t n = (row_tiles + kRowTiles * kUnroll - 1) / (kRowTiles * kUnroll);
+int launch(const char* who, void (*kernel)(P...), int64_t items, int per_thread, cudaStream_t s,
+           A... args) {
+  const int64_t per_block = static_cast<int64_t>(kLanes) * per_thread;
+  const int64_t n = (items + per_block - 1) / per_block;
   if (n > 0x7fffffffLL) return fail(AOTK_ERR_UNSUPPORTED, "%s: too many elements", who);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(n), 1, 1);
@@ -242,51 +319,41 @@ int launch(const char* who, void (*kernel)(P...), int64_t row_tiles, cudaStream_
   return check_launch(who);
 }
 
-Walk walk_of(int64_t cols) {
-  const int tiles_k = static_cast<int>((cols + 127) / 128);
-  return Walk{tiles_k, kRowTiles / tiles_k, kRowTiles % tiles_k};
+// Rows of whole 128-column scale tiles in items of `elements`.
+Walk walk_of(int64_t cols, int elements) {
+  const int items_k = static_cast<int>((cols + 127) / 128) * (128 / elements);
+  return Walk{items_k, kLanes / items_k, kLanes % items_k};
 }
 
-// Rows of 32 columns are 64 or 128 bytes, so the base and the row stride decide.
-template <typename T>
-int access_of(const void* p, int64_t stride) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * sizeof(T));
-  if (sizeof(T) == 4 && bits % 32 == 0) return kWide;
-  return bits % 16 == 0 ? kVectors : kElements;
+bool aligned32(const void* p, int64_t row_bytes) {
+  return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(row_bytes)) % 32 == 0;
 }
 
 template <typename T>
 int quantize(void* codes, void* scales, const void* x, int64_t stride, int64_t rows, int64_t cols,
              cudaStream_t s) {
-  const char* who = "aotk_mxfp4_quantize";
-  const Walk walk = walk_of(cols);
+  const Walk walk = walk_of(cols, 32);
   const int64_t padded = (rows + 127) / 128 * 128;
   auto run = [&](auto kernel) {
-    return launch(who, kernel, padded * walk.tiles_k, s, static_cast<uint8_t*>(codes),
-                  static_cast<uint8_t*>(scales), static_cast<const T*>(x), stride, rows, padded,
-                  static_cast<int>(cols), walk);
+    return launch("aotk_mxfp4_quantize", kernel, padded * walk.items_k, kItems<T>, s,
+                  static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
+                  static_cast<const T*>(x), stride, rows, padded, static_cast<int>(cols), walk);
   };
-  const int access = access_of<T>(x, rows > 1 ? stride : 0);
-  if constexpr (sizeof(T) == 4)
-    if (access == kWide) return run(quantize_kernel<T, kWide>);
-  return access == kVectors ? run(quantize_kernel<T, kVectors>) : run(quantize_kernel<T, kElements>);
+  return aligned32(x, rows > 1 ? stride * static_cast<int64_t>(sizeof(T)) : 0)
+             ? run(quantize_kernel<T, true>)
+             : run(quantize_kernel<T, false>);
 }
 
 template <typename T>
 int dequantize(void* out, const void* codes, const void* scales, int64_t rows, int64_t cols,
                cudaStream_t s) {
-  const char* who = "aotk_mxfp4_dequantize";
-  const Walk walk = walk_of(cols);
+  const Walk walk = walk_of(cols, kOutItem<T>);
   auto run = [&](auto kernel) {
-    return launch(who, kernel, rows * walk.tiles_k, s, static_cast<T*>(out),
+    return launch("aotk_mxfp4_dequantize", kernel, rows * walk.items_k, kOutUnroll, s, static_cast<T*>(out),
                   static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows,
                   static_cast<int>(cols), walk);
   };
-  const int access = access_of<T>(out, 0);
-  if constexpr (sizeof(T) == 4)
-    if (access == kWide) return run(dequantize_kernel<T, kWide>);
-  return access == kVectors ? run(dequantize_kernel<T, kVectors>)
-                            : run(dequantize_kernel<T, kElements>);
+  return aligned32(out, 0) ? run(dequantize_kernel<T, true>) : run(dequantize_kernel<T, false>);
 }
 
 }  // namespace
