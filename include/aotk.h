@@ -361,7 +361,7 @@ AOTK_API int aotk_gemm_schedule(int64_t M, int64_t N, int64_t K, int elem_bytes,
  * kernel: 1 producer, 2 MMA, 4 epilogue, 64 peer / flag wait, 128 self-test,
  * 2048 K-split partials; skinny kernel: 8, 16, 32; CTA-pair kernel: 256,
  * 512, 1024; 4-bit product: 4096, 8192, 16384, for
- * M <= 128 32768, 65536, 131072.  Synchronises the device.  clear != 0 resets it to 0 after reading. */
+ * M <= 128 32768, 65536, 131072; sandwich norm: 262144.  Synchronises the device.  clear != 0 resets it to 0 after reading. */
 AOTK_API int aotk_watchdog_status(int device, uint32_t* status, int clear);
 
 /* Runs the kernels' bounded waits with nothing to wait for - an mbarrier

@@ -437,6 +437,7 @@ extern "C" int aotk_watchdog_status(int device, uint32_t* status, int clear) {
   if (st == AOTK_OK) st = tc2_watchdog(status, clear != 0);
   if (st == AOTK_OK) st = mxfp4_watchdog(status, clear != 0);
   if (st == AOTK_OK) st = mxfp4_skinny_watchdog(status, clear != 0);
+  if (st == AOTK_OK) st = norm_watchdog(status, clear != 0);
   cudaSetDevice(prev);
   return st;
 }

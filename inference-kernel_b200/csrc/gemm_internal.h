@@ -95,6 +95,7 @@ int watchdog_selftest(void* stream);
 int tc_watchdog(uint32_t* status, bool clear);
 int mxfp4_watchdog(uint32_t* status, bool clear);
 int mxfp4_skinny_watchdog(uint32_t* status, bool clear);
+int norm_watchdog(uint32_t* status, bool clear);  // sandwich_norm.cu
 int skinny_watchdog(uint32_t* status, bool clear);
 
 // Raises the dynamic shared-memory limit of `kernel` to `bytes` once per device.
