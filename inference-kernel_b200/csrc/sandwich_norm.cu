@@ -5,16 +5,21 @@
 // reads.  fp32 math; h and out are each rounded once (the second norm sees the
 // unrounded h, so no error of h's rounding enters out).
 //
-// The row lives in registers from its one read to its two writes, so 2 rows
-// are read and 2 written per row of the problem, which bounds the kernel by
-// HBM.  A row is owned by TPR threads with VPT accesses of E elements each
-// (16-byte vectors, or single elements where the row length or a pointer is
-// not a multiple of 16 bytes); the two sums meet through warp shuffles and
-// shared memory.  Longer rows take a kernel that reads the row again.
+// Two rows are read and two written per row of the problem, which bounds it by
+// HBM: the row lives in registers from its one read to its two writes, and the
+// two sums meet through warp shuffles and shared memory.  Three kernels:
+//   * sandwich_kernel: TPR threads per row hold it in registers, everything
+//     requested before the first sum: few rows, and rows of any length whose
+//     starts are not multiples of 16 bytes;
+//   * sandwich_ring_kernel: many rows of 1 to 32 KB, streamed through shared memory;
+//   * sandwich_long_kernel: rows that fit neither, or tensors that do not start
+//     on 16 bytes: the row is read three times.
 //
 // gate is [gate_rows, gate_cols]: gate_cols is the row length or 1, and row r
 // of the problem uses gate row r / (rows / gate_rows) - one row for all
 // (per channel), one for each sequence, or one for each token.
+#include <type_traits>
+
 #include "common.h"
 #include "gemm_internal.h"
 #include "sm100.cuh"
@@ -27,6 +32,7 @@ struct Gate {
   const void* ptr;       // null: no gate
   int64_t rows_per;      // rows of the problem per gate row
   int64_t row_stride;
+  int64_t total;         // elements
   int col_stride;        // 1, or 0 for one value per row
 };
 
@@ -48,7 +54,7 @@ struct Args {
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* buf) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = TPR < 32 ? TPR / 2 : 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if constexpr (TPR > 32) {
     constexpr int WPR = TPR / 32;
     const int warp = threadIdx.x / 32;
@@ -62,31 +68,49 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
   return v;
 }
 
-template <typename T, int E>
-struct Access;  // one access of E consecutive elements
-
+// Elements [pos + lo, pos + hi) of `base` in their places of a vector, one by one.
 template <typename T>
-struct Access<T, 1> {
-  T v;
-  __device__ __forceinline__ void load(const T* p) { v = *p; }
-  __device__ __forceinline__ void load_cached(const T* p) { v = *p; }
-  __device__ __forceinline__ void get(float* f) const { f[0] = Elem<T>::to_f(v); }
-  __device__ __forceinline__ static void store(T* p, const float* f) { *p = Elem<T>::from_f(f[0]); }
-};
+__device__ __forceinline__ uint4 gather(const T* base, int64_t pos, int lo, int hi) {
+  constexpr int E = Elem<T>::kPerVec;
+  float f[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] = e >= lo && e < hi ? Elem<T>::to_f(base[pos + e]) : 0.f;
+  return Elem<T>::pack(f);
+}
 
-template <typename T, int E>
-struct Access {
-  static_assert(E == Elem<T>::kPerVec, "16-byte accesses");
-  uint4 v;
-  __device__ __forceinline__ void load(const T* p) { v = ld_stream(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void load_cached(const T* p) {
-    v = ld_cached(reinterpret_cast<const uint4*>(p));
+// Elements [shift, shift + E) of the vectors a and b.
+template <typename T>
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int shift) {
+  uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const int words = shift * static_cast<int>(sizeof(T)) / 4;
+#pragma unroll
+  for (int i = 0; i < 6; ++i) r[i] = words & 2 ? r[i + 2] : r[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) r[i] = words & 1 ? r[i + 1] : r[i];
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t bits = (shift & 1) * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __funnelshift_r(r[i], r[i + 1], bits);
   }
-  __device__ __forceinline__ void get(float* f) const { Elem<T>::unpack(v, f); }
-  __device__ __forceinline__ static void store(T* p, const float* f) {
-    st_stream(reinterpret_cast<uint4*>(p), Elem<T>::pack(f));
-  }
-};
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Elements [pos, pos + E) of `base` [total], which starts on 16 bytes, for any
+// pos > -E.  Only those in [lo, hi) are wanted; where a vector would reach behind
+// the last element they are taken one by one.
+template <typename T>
+__device__ __forceinline__ uint4 load_shifted(const T* base, int64_t pos, int64_t total, int lo,
+                                              int hi) {
+  constexpr int E = Elem<T>::kPerVec;
+  const int shift = static_cast<int>(pos & (E - 1));
+  const int64_t q = (pos - shift) / E;
+  if ((q + (shift ? 2 : 1)) * E > total) return gather(base, pos, lo, hi);
+  const uint4* v = reinterpret_cast<const uint4*>(base) + q;
+  uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+  if (q >= 0) a = ld_cached(v);
+  if (shift) b = ld_cached(v + 1);
+  return shifted<T>(a, b, shift);
+}
 
 // Two fp32 operations per instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -109,100 +133,199 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
+// Elements of a weight kept in shared memory: whole vectors, one before and one behind.
+template <typename T>
+__host__ __device__ constexpr int kept_elements(int cols) {
+  constexpr int E = Elem<T>::kPerVec;
+  return (cols + E - 1) / E * E + 2 * E;
+}
+
+// Copies a weight [cols], which starts on 16 bytes, to `kept` behind one vector of
+// zeros, zeros behind it.  All threads; the caller synchronises.
+template <typename T>
+__device__ __forceinline__ void keep_weight(T* kept, const T* w, int cols, int threads) {
+  constexpr int E = Elem<T>::kPerVec;
+  const int full = cols / E;
+  for (int v = threadIdx.x; v < full; v += threads)
+    reinterpret_cast<uint4*>(kept)[1 + v] = ld_cached(reinterpret_cast<const uint4*>(w) + v);
+  if (threadIdx.x == 0) reinterpret_cast<uint4*>(kept)[0] = make_uint4(0u, 0u, 0u, 0u);
+  const int c = full * E + threadIdx.x;
+  if (threadIdx.x < kept_elements<T>(cols) - E - full * E)
+    kept[E + c] = c < cols ? w[c] : Elem<T>::from_f(0.f);
+}
+
 constexpr int threads_for(int tpr) { return tpr > 256 ? tpr : 256; }
 
-template <typename T, int E, int VPT, int TPR>
+// kShift: rows need not start on 16 bytes (the tensors do).  A thread's vectors
+// are those of the tensors, so the row's first and last may hold elements of its
+// neighbours, which count as zeros and are not written; the weights' elements are
+// shifted into the places of the row's.  They are read from shared memory, where
+// each block keeps them with a vector to spare at both ends (from global memory
+// the vectors at a row's end would have to be taken apart: 127 us against 45 for
+// 20000 x 1001 bf16), and blocks go on to further rows.
+template <typename T, bool kShift, int VPT, int TPR>
 __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T> a) {
+  constexpr int E = Elem<T>::kPerVec;
+  constexpr int P = E / 2;  // pairs per vector
   constexpr int kThreads = threads_for(TPR);
   constexpr int RPB = kThreads / TPR;
+  // With 1024 threads the registers hold the row, but not its weights too.
+  constexpr bool kEarly = TPR < 1024;
   __shared__ float buf[2][kThreads / 32];
+  extern __shared__ __align__(16) uint8_t spare[];  // kShift: post, pre, one gate row
   const int t = threadIdx.x % TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
-  const bool live = row < a.rows;
-  const int64_t off = (live ? row : 0) * static_cast<int64_t>(a.cols);
+  const int64_t total = a.rows * static_cast<int64_t>(a.cols);
+  const T* gate = static_cast<const T*>(a.gate.ptr);
+  const bool gate_cols = gate != nullptr && a.gate.col_stride;
+  const bool gate_kept = kShift && gate_cols && a.gate.total == a.cols;
+  const int room = kept_elements<T>(a.cols);
+  T* kept = reinterpret_cast<T*>(spare);
 
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
-  const T* gate = static_cast<const T*>(a.gate.ptr);
-  if (gate != nullptr && live) gate += row / a.gate.rows_per * a.gate.row_stride;
+  if constexpr (kShift) {
+    keep_weight(kept, a.post, a.cols, kThreads);
+    keep_weight(kept + room, a.pre, a.cols, kThreads);
+    if (gate_kept) keep_weight(kept + 2 * room, gate, a.cols, kThreads);
+    __syncthreads();
+  }
+  // One pass unless kShift.
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPB; row0 < a.rows;
+       row0 += static_cast<int64_t>(gridDim.x) * RPB) {
+  const int64_t row = row0 + threadIdx.x / TPR;
+  const bool live = row < a.rows;
+  const int64_t off = (live ? row : 0) * static_cast<int64_t>(a.cols);
+  const int skip = kShift ? static_cast<int>(off & (E - 1)) : 0;
+  const int nv = live ? (skip + a.cols + E - 1) / E : 0;
+  const int64_t gate_at = live ? row / a.gate.rows_per * a.gate.row_stride : 0;
+  const float g_row = gate != nullptr && !gate_cols ? Elem<T>::to_f(gate[gate_at]) : 1.f;
 
-  // Everything that the row needs is requested before the first sum.
-  Access<T, E> x[VPT], res[VPT], post[VPT], pre[VPT], g[VPT];
-  float g_row = 1.f;
+  auto column = [&](int i) { return (t + i * TPR) * E - skip; };  // of element 0
+  auto used = [&](int i) { return t + i * TPR < nv; };
+  auto first = [&](int c) { return kShift && c < 0 ? -c : 0; };
+  auto last = [&](int c) { return kShift && a.cols - c < E ? a.cols - c : E; };
+  auto row_vec = [&](const T* p, int c) {
+    if constexpr (kShift)
+      if (off + c + E > total) return gather(p, off + c, first(c), last(c));
+    return ld_stream(reinterpret_cast<const uint4*>(p + off + c));
+  };
+  auto col_vec = [&](const T* p, int c, int which) {  // of a weight, or the only gate row
+    if constexpr (kShift) {
+      // Element c is at E + c there: the same shift for the whole row.
+      const uint4* v = reinterpret_cast<const uint4*>(kept + which * room) + (c + skip) / E;
+      return skip ? shifted<T>(v[0], v[1], E - skip) : v[1];
+    }
+    return ld_cached(reinterpret_cast<const uint4*>(p + c));
+  };
+  auto gate_vec = [&](int c) {
+    if constexpr (kShift) {
+      if (gate_kept) return col_vec(gate, c, 2);
+      return load_shifted(gate, gate_at + c, a.gate.total, first(c), last(c));
+    }
+    return ld_cached(reinterpret_cast<const uint4*>(gate + gate_at + c));
+  };
+  auto write = [&](T* p, int c, const float2* f) {
+    const uint4 v = Elem<T>::pack(&f[0].x);
+    const int lo = first(c), hi = last(c);
+    if (!kShift || (lo == 0 && hi == E)) {
+      st_stream(reinterpret_cast<uint4*>(p + off + c), v);
+    } else {
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (k >= lo && k < hi) p[off + c + k] = e[k];
+    }
+  };
+  auto mask = [&](int c, float2* f) {  // zeros where the row is not
+    if constexpr (kShift) {
+      const int lo = first(c), hi = last(c);
+      if (lo > 0 || hi < E) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          if (2 * k < lo || 2 * k >= hi) f[k].x = 0.f;
+          if (2 * k + 1 < lo || 2 * k + 1 >= hi) f[k].y = 0.f;
+        }
+      }
+    }
+  };
+
+  uint4 x[VPT], res[VPT], post[VPT], pre[VPT], g[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int c = (t + i * TPR) * E;
-    if (live && c < a.cols) {
-      x[i].load(a.x + off + c);
-      res[i].load(a.residual + off + c);
+    if (used(i)) {
+      x[i] = row_vec(a.x, column(i));
+      res[i] = row_vec(a.residual, column(i));
     }
   }
+  auto load_post = [&](int i) {
+    post[i] = col_vec(a.post, column(i), 0);
+    if (gate_cols) g[i] = gate_vec(column(i));
+  };
+  auto load_pre = [&](int i) { pre[i] = col_vec(a.pre, column(i), 1); };
+  if constexpr (kEarly) {
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = (t + i * TPR) * E;
-    if (live && c < a.cols) {
-      post[i].load_cached(a.post + c);
-      pre[i].load_cached(a.pre + c);
-      if (gate != nullptr && a.gate.col_stride) g[i].load_cached(gate + c);
+    for (int i = 0; i < VPT; ++i) {
+      if (used(i)) {
+        load_post(i);
+        load_pre(i);
+      }
     }
   }
-  if (gate != nullptr && live && !a.gate.col_stride) g_row = Elem<T>::to_f(gate[0]);
-  const bool gate_cols = gate != nullptr && a.gate.col_stride;
 
-  float ss = 0.f;
+  float2 h[VPT][P];  // x, then h
+  float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (live && (t + i * TPR) * E < a.cols) {
-      float f[E];
-      x[i].get(f);
+    if (used(i)) {
+      Elem<T>::unpack(x[i], &h[i][0].x);
+      mask(column(i), h[i]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
+      for (int e = 0; e < P; ++e) ss = fma2(h[i][e], h[i][e], ss);
     }
   }
-  ss = row_sum<TPR>(ss, buf[0]);
-  const float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  const float sum = row_sum<TPR>(ss.x + ss.y, buf[0]);
+  const float inv = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
 
-  float h[VPT][E];
-  ss = 0.f;
+  ss = make_float2(0.f, 0.f);
+  const float scale = inv * g_row;
+  const float2 scale2 = make_float2(scale, scale), alpha2 = make_float2(a.alpha, a.alpha);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int c = (t + i * TPR) * E;
-    if (live && c < a.cols) {
-      float r[E], w[E];
-      x[i].get(h[i]);
-      res[i].get(r);
-      post[i].get(w);
+    if (used(i)) {
+      if constexpr (!kEarly) load_post(i);
+      float2 w[P];
+      Elem<T>::unpack(post[i], &w[0].x);
 #pragma unroll
-      for (int e = 0; e < E; ++e) h[i][e] = h[i][e] * inv * w[e];
+      for (int e = 0; e < P; ++e) h[i][e] = mul2(mul2(h[i][e], scale2), w[e]);
       if (gate_cols) {
-        float gf[E];
-        g[i].get(gf);
+        Elem<T>::unpack(g[i], &w[0].x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) h[i][e] *= gf[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[i][e] *= g_row;
+        for (int e = 0; e < P; ++e) h[i][e] = mul2(h[i][e], w[e]);
       }
+      Elem<T>::unpack(res[i], &w[0].x);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        h[i][e] = fmaf(a.alpha, r[e], h[i][e]);
-        ss = fmaf(h[i][e], h[i][e], ss);
-      }
-      Access<T, E>::store(a.h_out + off + c, h[i]);
+      for (int e = 0; e < P; ++e) h[i][e] = fma2(alpha2, w[e], h[i][e]);
+      mask(column(i), h[i]);
+#pragma unroll
+      for (int e = 0; e < P; ++e) ss = fma2(h[i][e], h[i][e], ss);
+      write(a.h_out, column(i), h[i]);
     }
   }
-  ss = row_sum<TPR>(ss, buf[1]);
-  const float inv_h = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  const float sum_h = row_sum<TPR>(ss.x + ss.y, buf[1]);
+  const float inv_h = rsqrtf(sum_h / static_cast<float>(a.cols) + a.eps);
+  const float2 inv_h2 = make_float2(inv_h, inv_h);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int c = (t + i * TPR) * E;
-    if (live && c < a.cols) {
-      float w[E];
-      pre[i].get(w);
+    if (used(i)) {
+      if constexpr (!kEarly) load_pre(i);
+      float2 w[P];
+      Elem<T>::unpack(pre[i], &w[0].x);
 #pragma unroll
-      for (int e = 0; e < E; ++e) w[e] *= h[i][e] * inv_h;
-      Access<T, E>::store(a.out + off + c, w);
+      for (int e = 0; e < P; ++e) w[e] = mul2(mul2(h[i][e], inv_h2), w[e]);
+      write(a.out, column(i), w);
     }
+  }
+  if constexpr (!kShift) break;
   }
 }
 
@@ -217,11 +340,11 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
 constexpr int kRingThreads = 512;
 constexpr int kRingBytes = 196608;
 constexpr int kMaxStages = 8;
-#ifndef RMIN
-#define RMIN 1024
-#define RTOT (1<<20)
+#ifndef RTOT
+#define RTOT (1 << 20)
 #endif
-constexpr int64_t kRingMinRow = RMIN, kRingMinTotal = RTOT;
+constexpr int64_t kRingMinRow = 1024, kRingMaxRow = 32768, kRingMinTotal = RTOT;
+constexpr int64_t kRingMaxShift = 16384;  // with the weights beside the ring
 
 __device__ unsigned g_norm_watchdog;
 enum : unsigned { kWdRow = 262144u };
@@ -252,7 +375,19 @@ __device__ __forceinline__ float group_sum(float v, float* buf, int group, int t
   return v;
 }
 
-template <typename T, int VPT, int TPR>
+template <int TPR>
+__device__ __forceinline__ void group_sync(int group) {
+  if constexpr (TPR == 32)
+    __syncwarp();
+  else
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+}
+
+// kShift: rows need not start on 16 bytes (the tensors do).  The copies take the
+// vectors around a row, a thread works on those, and the row's first and last are
+// written element by element; weights come from shared memory, shifted into the
+// places of the row's elements.
+template <typename T, bool kShift, int VPT, int TPR>
 __global__ void __launch_bounds__(kRingThreads, 1)
     sandwich_ring_kernel(const Args<T> a, int stages, int pitch) {
   using namespace sm100;
@@ -260,16 +395,23 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   constexpr int P = E / 2;  // pairs per vector
   constexpr int G = kRingThreads / TPR;
   constexpr int WPR = TPR / 32;
-  extern __shared__ __align__(16) uint8_t ring[];  // [G][stages][x, residual][pitch]
+  extern __shared__ __align__(16) uint8_t ring[];  // [G][stages][x, residual][pitch], then weights
   __shared__ float partial[G][2][WPR];
   __shared__ __align__(8) uint64_t bars[G][kMaxStages];
+  __shared__ __align__(16) uint4 ends[kShift ? G : 1][2][2];  // [h, out][first, last vector]
   __shared__ int abort_flag;
   const int group = threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   const int64_t step = static_cast<int64_t>(gridDim.x) * G;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * G + group;
+  const int64_t first_row = static_cast<int64_t>(blockIdx.x) * G + group;
+  const int64_t total = a.rows * static_cast<int64_t>(a.cols);
   uint8_t* mine = ring + static_cast<int64_t>(group) * stages * 2 * pitch;
   const uint32_t bar0 = smem_addr(bars[group]);
+  const T* gate = static_cast<const T*>(a.gate.ptr);
+  const bool gate_cols = gate != nullptr && a.gate.col_stride;
+  const bool gate_kept = kShift && gate_cols && a.gate.total == a.cols;
+  const int room = kept_elements<T>(a.cols);
+  T* kept = reinterpret_cast<T*>(ring + static_cast<int64_t>(G) * stages * 2 * pitch);
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -281,65 +423,126 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   __syncthreads();
   pdl_wait_prior();
 
+  // The row's vectors: from the one that its first element is in to the one that
+  // its last is in, or the tensor's last whole one.
   auto request = [&](int64_t row, int stage) {  // one thread
-    const uint32_t bytes = static_cast<uint32_t>(a.cols) * sizeof(T);
+    const int64_t v0 = row * a.cols / E;
+    uint32_t vectors = static_cast<uint32_t>(a.cols / E);
+    if constexpr (kShift) {
+      int64_t v1 = (row + 1) * a.cols / E;
+      if (v1 * E < (row + 1) * a.cols && (v1 + 1) * E <= total) ++v1;
+      vectors = static_cast<uint32_t>(v1 - v0);
+    }
+    const uint32_t bytes = vectors * 16u;
     const uint32_t bar = bar0 + 8u * stage;
     const uint32_t dst = smem_addr(mine + static_cast<int64_t>(stage) * 2 * pitch);
     mbar_arrive_expect_tx(bar, 2 * bytes);
-    bulk_load(dst, a.x + row * a.cols, bytes, bar);
-    bulk_load(dst + pitch, a.residual + row * a.cols, bytes, bar);
+    bulk_load(dst, a.x + v0 * E, bytes, bar);
+    bulk_load(dst + pitch, a.residual + v0 * E, bytes, bar);
   };
   if (t == 0)
-    for (int k = 0; k < stages && first + k * step < a.rows; ++k) request(first + k * step, k);
+    for (int k = 0; k < stages && first_row + k * step < a.rows; ++k)
+      request(first_row + k * step, k);
 
-  // A thread's columns are the same in every row, so their weights stay in
-  // registers (from L2 they would be as many bytes per row as x and the
-  // residual), and so does the gate until its row changes.
-  const T* gate = static_cast<const T*>(a.gate.ptr);
-  const bool gate_cols = gate != nullptr && a.gate.col_stride;
+  // Rows that start on 16 bytes: a thread's columns are the same in every row, so
+  // their weights stay in registers (from L2 they would be as many bytes per row
+  // as x and the residual), and so does the gate until its row changes.
   uint4 post[VPT], pre[VPT], g[VPT];
   float g_row = 1.f;
   int64_t g_at = -1;
+  if constexpr (kShift) {
+    keep_weight(kept, a.post, a.cols, kRingThreads);
+    keep_weight(kept + room, a.pre, a.cols, kRingThreads);
+    if (gate_kept) keep_weight(kept + 2 * room, gate, a.cols, kRingThreads);
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = (t + i * TPR) * E;
-    if (c < a.cols) {
-      post[i] = ld_cached(reinterpret_cast<const uint4*>(a.post + c));
-      pre[i] = ld_cached(reinterpret_cast<const uint4*>(a.pre + c));
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (t + i * TPR) * E;
+      if (c < a.cols) {
+        post[i] = ld_cached(reinterpret_cast<const uint4*>(a.post + c));
+        pre[i] = ld_cached(reinterpret_cast<const uint4*>(a.pre + c));
+      }
     }
   }
 
   int stage = 0;
   uint32_t phase = 0;
-  for (int64_t row = first; row < a.rows; row += step) {
+  for (int64_t row = first_row; row < a.rows; row += step) {
+    const int64_t off = row * a.cols;
+    const int skip = kShift ? static_cast<int>(off & (E - 1)) : 0;
+    const int nv = (skip + a.cols + E - 1) / E;
+    auto column = [&](int i) { return (t + i * TPR) * E - skip; };  // of element 0
+    auto used = [&](int i) { return t + i * TPR < nv; };
+    auto first = [&](int c) { return kShift && c < 0 ? -c : 0; };
+    auto last = [&](int c) { return kShift && a.cols - c < E ? a.cols - c : E; };
+    auto kept_vec = [&](int which, int i) {
+      const uint4* v = reinterpret_cast<const uint4*>(kept + which * room) + t + i * TPR;
+      return skip ? shifted<T>(v[0], v[1], E - skip) : v[1];
+    };
+    auto mask = [&](int c, float2* f) {  // zeros where the row is not
+      if constexpr (kShift) {
+        const int lo = first(c), hi = last(c);
+        if (lo > 0 || hi < E) {
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            if (2 * k < lo || 2 * k >= hi) f[k].x = 0.f;
+            if (2 * k + 1 < lo || 2 * k + 1 >= hi) f[k].y = 0.f;
+          }
+        }
+      }
+    };
+    // A whole vector goes to its place, one that the row shares to `ends`.
+    auto write = [&](T* p, int which, int i, const float2* f) {
+      const uint4 v = Elem<T>::pack(&f[0].x);
+      const int c = column(i);
+      if (kShift && (c < 0 || c + E > a.cols))
+        ends[kShift ? group : 0][which][c < 0 ? 0 : 1] = v;
+      else
+        st_stream(reinterpret_cast<uint4*>(p + off + c), v);
+    };
     if (gate != nullptr) {
       const int64_t at = row / a.gate.rows_per;
       if (at != g_at) {
         g_at = at;
-        const T* gr = gate + at * a.gate.row_stride;
-        if (gate_cols) {
+        if (!gate_cols) {
+          g_row = Elem<T>::to_f(gate[at * a.gate.row_stride]);
+        } else if constexpr (!kShift) {
+          const T* gr = gate + at * a.gate.row_stride;
 #pragma unroll
           for (int i = 0; i < VPT; ++i) {
             const int c = (t + i * TPR) * E;
             if (c < a.cols) g[i] = ld_cached(reinterpret_cast<const uint4*>(gr + c));
           }
-        } else {
-          g_row = Elem<T>::to_f(*gr);
+        }
+      }
+      if constexpr (kShift) {
+        if (gate_cols && !gate_kept) {
+#pragma unroll
+          for (int i = 0; i < VPT; ++i)
+            if (used(i))
+              g[i] = load_shifted(gate, at * a.cols + column(i), a.gate.total, first(column(i)),
+                                  last(column(i)));
         }
       }
     }
     const uint4* xs = reinterpret_cast<const uint4*>(mine + static_cast<int64_t>(stage) * 2 * pitch);
     const uint4* rs = reinterpret_cast<const uint4*>(mine + (static_cast<int64_t>(stage) * 2 + 1) * pitch);
-    T* h_row = a.h_out + row * a.cols;
-    T* o_row = a.out + row * a.cols;
+    // The tensor's last elements may lie behind its last whole vector.
+    const bool cut = kShift && off + a.cols == total && total % E != 0;
+    auto row_vec = [&](const uint4* sm, const T* gm, int i) {
+      if (cut && t + i * TPR == nv - 1) return gather(gm, off + column(i), first(column(i)), last(column(i)));
+      return sm[t + i * TPR];
+    };
     bool bad = !mbar_wait_bounded(bar0 + 8u * stage, phase, &abort_flag, &g_norm_watchdog, kWdRow);
 
     float2 h[VPT][P];  // x, then h
     float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      if ((t + i * TPR) * E < a.cols) {
-        Elem<T>::unpack(xs[t + i * TPR], &h[i][0].x);
+      if (used(i)) {
+        Elem<T>::unpack(row_vec(xs, a.x, i), &h[i][0].x);
+        mask(column(i), h[i]);
 #pragma unroll
         for (int e = 0; e < P; ++e) ss = fma2(h[i][e], h[i][e], ss);
       }
@@ -353,24 +556,23 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     const float2 scale2 = make_float2(scale, scale), alpha2 = make_float2(a.alpha, a.alpha);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = (t + i * TPR) * E;
-      if (c < a.cols) {
+      if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(post[i], &w[0].x);
+        Elem<T>::unpack(kShift ? kept_vec(0, i) : post[i], &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) h[i][e] = mul2(mul2(h[i][e], scale2), w[e]);
         if (gate_cols) {
-          Elem<T>::unpack(g[i], &w[0].x);
+          Elem<T>::unpack(gate_kept ? kept_vec(2, i) : g[i], &w[0].x);
 #pragma unroll
           for (int e = 0; e < P; ++e) h[i][e] = mul2(h[i][e], w[e]);
         }
-        Elem<T>::unpack(rs[t + i * TPR], &w[0].x);
+        Elem<T>::unpack(row_vec(rs, a.residual, i), &w[0].x);
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-          h[i][e] = fma2(alpha2, w[e], h[i][e]);
-          ss = fma2(h[i][e], h[i][e], ss);
-        }
-        st_stream(reinterpret_cast<uint4*>(h_row + c), Elem<T>::pack(&h[i][0].x));
+        for (int e = 0; e < P; ++e) h[i][e] = fma2(alpha2, w[e], h[i][e]);
+        mask(column(i), h[i]);
+#pragma unroll
+        for (int e = 0; e < P; ++e) ss = fma2(h[i][e], h[i][e], ss);
+        write(a.h_out, 0, i, h[i]);
       }
     }
     const float sum_h = group_sum<TPR>(ss.x + ss.y, partial[group][1], group, t, bad);
@@ -380,14 +582,25 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     const float2 inv_h2 = make_float2(inv_h, inv_h);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = (t + i * TPR) * E;
-      if (c < a.cols) {
+      if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(pre[i], &w[0].x);
+        Elem<T>::unpack(kShift ? kept_vec(1, i) : pre[i], &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) w[e] = mul2(mul2(h[i][e], inv_h2), w[e]);
-        st_stream(reinterpret_cast<uint4*>(o_row + c), Elem<T>::pack(&w[0].x));
+        write(a.out, 1, i, w);
       }
+    }
+    if constexpr (kShift) {
+      // One lane per element of the first and the last vector, if they are shared.
+      group_sync<TPR>(group);
+      if (t < 4 * E) {
+        const int which = t / (2 * E), end = t / E % 2, e = t % E;
+        const int c = (end ? nv - 1 : 0) * E - skip;
+        if ((end ? c + E > a.cols : c < 0) && c + e >= 0 && c + e < a.cols)
+          (which ? a.out : a.h_out)[off + c + e] =
+              reinterpret_cast<const T*>(&ends[kShift ? group : 0][which][end])[e];
+      }
+      group_sync<TPR>(group);
     }
     if (++stage == stages) {
       stage = 0;
@@ -399,92 +612,158 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int k = 0; k < stages; ++k) mbar_drain(bar0 + 8u * k, phase);
 }
 
-// Any row length: one block per row; h is computed again from its inputs for
-// the output pass, so that it is never rounded in between.
-template <typename T>
-__global__ void __launch_bounds__(256) sandwich_long_kernel(const Args<T> a) {
-  __shared__ float buf[2][8];
+// Any row length and alignment: one block per row; h is computed again from its
+// inputs for the output pass, so that it is never rounded in between.
+constexpr int kLongThreads = 1024;
+
+template <typename T, int E>
+__global__ void __launch_bounds__(kLongThreads) sandwich_long_kernel(const Args<T> a) {
+  __shared__ float buf[2][kLongThreads / 32];
   const int64_t row = blockIdx.x;
   const int64_t off = row * a.cols;
+  sm100::pdl_launch_dependents();
+  sm100::pdl_wait_prior();
+  auto load = [](const T* p, float* f) {
+    if constexpr (E == 1)
+      f[0] = Elem<T>::to_f(*p);
+    else
+      Elem<T>::unpack(ld_cached(reinterpret_cast<const uint4*>(p)), f);
+  };
+  auto store = [](T* p, const float* f) {
+    if constexpr (E == 1)
+      *p = Elem<T>::from_f(f[0]);
+    else
+      st_stream(reinterpret_cast<uint4*>(p), Elem<T>::pack(f));
+  };
+  const int step = kLongThreads * E;
   float ss = 0.f;
-  for (int c = threadIdx.x; c < a.cols; c += 256) {
-    const float f = Elem<T>::to_f(a.x[off + c]);
-    ss = fmaf(f, f, ss);
+  for (int64_t c = threadIdx.x * E; c < a.cols; c += step) {
+    float f[E];
+    load(a.x + off + c, f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
   }
-  ss = row_sum<256>(ss, buf[0]);
+  ss = row_sum<kLongThreads>(ss, buf[0]);
   const float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
   const T* gate = static_cast<const T*>(a.gate.ptr);
   if (gate != nullptr) gate += row / a.gate.rows_per * a.gate.row_stride;
-  auto h_at = [&](int c) {
-    float v = Elem<T>::to_f(a.x[off + c]) * inv * Elem<T>::to_f(a.post[c]);
-    if (gate != nullptr) v *= Elem<T>::to_f(gate[static_cast<int64_t>(c) * a.gate.col_stride]);
-    return fmaf(a.alpha, Elem<T>::to_f(a.residual[off + c]), v);
+  const bool gate_cols = gate != nullptr && a.gate.col_stride;
+  const float scale = gate != nullptr && !gate_cols ? inv * Elem<T>::to_f(*gate) : inv;
+  auto h_at = [&](int64_t c, float* h) {
+    float w[E];
+    load(a.x + off + c, h);
+    load(a.post + c, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = h[e] * scale * w[e];
+    if (gate_cols) {
+      load(gate + c, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) h[e] *= w[e];
+    }
+    load(a.residual + off + c, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = fmaf(a.alpha, w[e], h[e]);
   };
   ss = 0.f;
-  for (int c = threadIdx.x; c < a.cols; c += 256) {
-    const float h = h_at(c);
-    ss = fmaf(h, h, ss);
+  for (int64_t c = threadIdx.x * E; c < a.cols; c += step) {
+    float h[E];
+    h_at(c, h);
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss = fmaf(h[e], h[e], ss);
   }
-  ss = row_sum<256>(ss, buf[1]);
+  ss = row_sum<kLongThreads>(ss, buf[1]);
   const float inv_h = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
-  for (int c = threadIdx.x; c < a.cols; c += 256) {
-    const float h = h_at(c);
-    a.h_out[off + c] = Elem<T>::from_f(h);
-    a.out[off + c] = Elem<T>::from_f(h * inv_h * Elem<T>::to_f(a.pre[c]));
+  for (int64_t c = threadIdx.x * E; c < a.cols; c += step) {
+    float h[E], w[E];
+    h_at(c, h);
+    store(a.h_out + off + c, h);
+    load(a.pre + c, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] *= h[e] * inv_h;
+    store(a.out + off + c, w);
   }
 }
 
-template <typename T, int E, int VPT, int TPR>
-int launch_rows(const Args<T>& a, cudaStream_t s) {
-  constexpr int kThreads = threads_for(TPR);
-  const int64_t blocks = (a.rows + kThreads / TPR - 1) / (kThreads / TPR);
+template <typename T>
+int launch_kernel(void (*kernel)(const Args<T>), const Args<T>& a, int64_t blocks, int threads,
+                  size_t smem, cudaStream_t s) {
   if (blocks > 0x7fffffffLL)
     return fail(AOTK_ERR_INVALID_ARGUMENT, "aotk_sandwich_rmsnorm: too many rows");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, sandwich_kernel<T, E, VPT, TPR>, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e != cudaSuccess)
     return fail(AOTK_ERR_CUDA, "aotk_sandwich_rmsnorm launch: %s", cudaGetErrorString(e));
   return check_launch("aotk_sandwich_rmsnorm");
 }
 
-template <typename T, int E>
-int launch_access(const Args<T>& a, cudaStream_t s) {
-    constexpr int V = E == 1 ? 8 : 4;  // accesses per thread
-  const int n = a.cols / E;
-  if (n <= 32) return launch_rows<T, E, 1, 32>(a, s);
-  if (n <= V * 32) return launch_rows<T, E, V, 32>(a, s);
-  if (n <= V * 64) return launch_rows<T, E, V, 64>(a, s);
-  if (n <= V * 128) return launch_rows<T, E, V, 128>(a, s);
-  if (n <= V * 256) return launch_rows<T, E, V, 256>(a, s);
-  if (n <= V * 512) return launch_rows<T, E, V, 512>(a, s);
-  if (n <= V * 1024) return launch_rows<T, E, V, 1024>(a, s);
-  if (a.rows > 0x7fffffffLL)
-    return fail(AOTK_ERR_INVALID_ARGUMENT, "aotk_sandwich_rmsnorm: too many rows");
-  sandwich_long_kernel<T><<<static_cast<unsigned>(a.rows), 256, 0, s>>>(a);
-  return check_launch("aotk_sandwich_rmsnorm");
+template <typename T, bool kShift, int VPT, int TPR>
+int launch_rows(const Args<T>& a, cudaStream_t s) {
+  constexpr int kThreads = threads_for(TPR);
+  auto kernel = sandwich_kernel<T, kShift, VPT, TPR>;
+  int64_t blocks = (a.rows + kThreads / TPR - 1) / (kThreads / TPR);
+  size_t smem = 0;
+  if constexpr (kShift) {
+    DeviceInfo info;
+    if (int st = current_device_info(&info)) return st;
+    smem = 3 * sizeof(T) * static_cast<size_t>(kept_elements<T>(a.cols));
+    // The largest room this kernel may need: VPT * TPR vectors of a row.
+    constexpr size_t most = 3 * 16 * (static_cast<size_t>(VPT) * TPR + 2);
+    if (most > 48 * 1024)
+      if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), most, info)) return st;
+    const int64_t resident = static_cast<int64_t>(info.sm_count) *
+                             (kThreads > 256 || smem > 100 * 1024 ? 1 : smem > 64 * 1024 ? 2 : 3);
+    if (blocks > resident) blocks = resident;
+  }
+  return launch_kernel<T>(kernel, a, blocks, kThreads, smem, s);
 }
 
-template <typename T, int VPT, int TPR>
+template <typename T, int E>
+int launch_long(const Args<T>& a, cudaStream_t s) {
+  return launch_kernel<T>(sandwich_long_kernel<T, E>, a, a.rows, kLongThreads, 0, s);
+}
+
+// The smallest group of threads that holds a row in at most four vectors each.
+template <typename T, bool kShift>
+int dispatch_rows(const Args<T>& a, cudaStream_t s) {
+  constexpr int E = Elem<T>::kPerVec;
+  const int64_t n = (static_cast<int64_t>(a.cols) + (kShift ? 2 * (E - 1) : 0)) / E;  // at most
+  if (n <= 8) return launch_rows<T, kShift, 1, 8>(a, s);
+  if (n <= 16) return launch_rows<T, kShift, 2, 8>(a, s);
+  if (n <= 32) return launch_rows<T, kShift, 4, 8>(a, s);
+  if (n <= 64) return launch_rows<T, kShift, 2, 32>(a, s);
+  if (n <= 128) return launch_rows<T, kShift, 4, 32>(a, s);
+  if (n <= 256) return launch_rows<T, kShift, 4, 64>(a, s);
+  if (n <= 512) return launch_rows<T, kShift, 4, 128>(a, s);
+  if (n <= 1024) return launch_rows<T, kShift, 4, 256>(a, s);
+  if (n <= 2048) return launch_rows<T, kShift, 4, 512>(a, s);
+  if (n <= 4096) return launch_rows<T, kShift, 4, 1024>(a, s);
+  return kShift ? launch_long<T, 1>(a, s) : launch_long<T, E>(a, s);
+}
+
+template <typename T, bool kShift, int VPT, int TPR>
 int launch_ring(const Args<T>& a, cudaStream_t s, const DeviceInfo& info) {
   constexpr int G = kRingThreads / TPR;
-  const int pitch = a.cols * static_cast<int>(sizeof(T));
-  int stages = kRingBytes / (G * 2 * pitch);
+  constexpr int E = Elem<T>::kPerVec;
+  const int pitch = ((a.cols + E - 1) / E + (kShift ? 1 : 0)) * 16;
+  const int weights = kShift ? 3 * static_cast<int>(sizeof(T)) * kept_elements<T>(a.cols) : 0;
+  int stages = (kRingBytes - weights) / (G * 2 * pitch);
   if (stages > kMaxStages) stages = kMaxStages;
-  auto kernel = sandwich_ring_kernel<T, VPT, TPR>;
+  auto kernel = sandwich_ring_kernel<T, kShift, VPT, TPR>;
   if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes, info)) return st;
   const int64_t groups = (a.rows + G - 1) / G;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(groups < info.sm_count ? groups : info.sm_count), 1, 1);
   cfg.blockDim = dim3(kRingThreads, 1, 1);
-  cfg.dynamicSmemBytes = static_cast<size_t>(G) * stages * 2 * pitch;
+  cfg.dynamicSmemBytes = static_cast<size_t>(G) * stages * 2 * pitch + weights;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -498,20 +777,21 @@ int launch_ring(const Args<T>& a, cudaStream_t s, const DeviceInfo& info) {
 }
 
 // The smallest group that holds a row in at most four vectors per thread.
-template <typename T>
+template <typename T, bool kShift>
 int dispatch_ring(const Args<T>& a, cudaStream_t s, const DeviceInfo& info) {
-  const int n = a.cols / Elem<T>::kPerVec;
-  if (n <= 2 * 32) return launch_ring<T, 2, 32>(a, s, info);
-  if (n <= 3 * 32) return launch_ring<T, 3, 32>(a, s, info);
-  if (n <= 4 * 32) return launch_ring<T, 4, 32>(a, s, info);
-  if (n <= 3 * 64) return launch_ring<T, 3, 64>(a, s, info);
-  if (n <= 4 * 64) return launch_ring<T, 4, 64>(a, s, info);
-  if (n <= 3 * 128) return launch_ring<T, 3, 128>(a, s, info);
-  if (n <= 4 * 128) return launch_ring<T, 4, 128>(a, s, info);
-  if (n <= 3 * 256) return launch_ring<T, 3, 256>(a, s, info);
-  if (n <= 4 * 256) return launch_ring<T, 4, 256>(a, s, info);
-  if (n <= 3 * 512) return launch_ring<T, 3, 512>(a, s, info);
-  return launch_ring<T, 4, 512>(a, s, info);
+  constexpr int E = Elem<T>::kPerVec;
+  const int n = (a.cols + (kShift ? 2 * (E - 1) : 0)) / E;  // at most
+  if (n <= 2 * 32) return launch_ring<T, kShift, 2, 32>(a, s, info);
+  if (n <= 3 * 32) return launch_ring<T, kShift, 3, 32>(a, s, info);
+  if (n <= 4 * 32) return launch_ring<T, kShift, 4, 32>(a, s, info);
+  if (n <= 3 * 64) return launch_ring<T, kShift, 3, 64>(a, s, info);
+  if (n <= 4 * 64) return launch_ring<T, kShift, 4, 64>(a, s, info);
+  if (n <= 3 * 128) return launch_ring<T, kShift, 3, 128>(a, s, info);
+  if (n <= 4 * 128) return launch_ring<T, kShift, 4, 128>(a, s, info);
+  if (n <= 3 * 256) return launch_ring<T, kShift, 3, 256>(a, s, info);
+  if (n <= 4 * 256) return launch_ring<T, kShift, 4, 256>(a, s, info);
+  if (n <= 3 * 512) return launch_ring<T, kShift, 3, 512>(a, s, info);
+  return launch_ring<T, kShift, 4, 512>(a, s, info);
 }
 
 template <typename T>
@@ -525,15 +805,17 @@ int launch(void* out, void* h_out, const void* x, const void* residual, const vo
                      static_cast<float>(eps),     rows,
                      static_cast<int>(cols)};
   constexpr int E = Elem<T>::kPerVec;
-  const bool vec = cols % E == 0 && aligned16(x) && aligned16(residual) && aligned16(post) &&
-                   aligned16(pre) && aligned16(out) && aligned16(h_out) && aligned16(gate.ptr);
-  // Rows of 1 to 32 KB, enough of them to fill the ring: the ring kernel.
+  if (!(aligned16(x) && aligned16(residual) && aligned16(post) && aligned16(pre) &&
+        aligned16(out) && aligned16(h_out) && aligned16(gate.ptr)))
+    return launch_long<T, 1>(a, s);
   DeviceInfo info;
   if (int st = current_device_info(&info)) return st;
+  const bool shift = cols % E != 0;
   const int64_t row_bytes = cols * static_cast<int64_t>(sizeof(T));
-  if (vec && row_bytes >= kRingMinRow && row_bytes <= 32768 && rows * row_bytes >= kRingMinTotal)
-    return dispatch_ring<T>(a, s, info);
-  return vec ? launch_access<T, E>(a, s) : launch_access<T, 1>(a, s);
+  if (row_bytes >= kRingMinRow && row_bytes <= (shift ? kRingMaxShift : kRingMaxRow) &&
+      rows * row_bytes >= kRingMinTotal)
+    return shift ? dispatch_ring<T, true>(a, s, info) : dispatch_ring<T, false>(a, s, info);
+  return shift ? dispatch_rows<T, true>(a, s) : dispatch_rows<T, false>(a, s);
 }
 
 }  // namespace
@@ -566,13 +848,13 @@ extern "C" int aotk_sandwich_rmsnorm(void* out, void* h_out, const void* x, cons
   if (!out || !h_out || !x || !residual || !post_weight || !pre_weight)
     return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   if (cols > 0x3fffffffLL) return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: row too long", who);
-  Gate g = {nullptr, 1, 0, 0};
+  Gate g = {nullptr, 1, 0, 0, 0};
   if (gate) {
     if (gate_rows < 1 || rows % gate_rows != 0 || (gate_cols != cols && gate_cols != 1))
       return fail(AOTK_ERR_INVALID_ARGUMENT,
                   "%s: gate [%lld, %lld] does not fit rows [%lld, %lld]", who, (long long)gate_rows,
                   (long long)gate_cols, (long long)rows, (long long)cols);
-    g = {gate, rows / gate_rows, gate_cols, gate_cols == cols ? 1 : 0};
+    g = {gate, rows / gate_rows, gate_cols, gate_rows * gate_cols, gate_cols == cols ? 1 : 0};
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {

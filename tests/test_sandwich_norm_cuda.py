@@ -71,6 +71,28 @@ def test_row_counts(rows, dtype):
     check(make((rows, 512), dtype, seed=rows), dtype, alpha=0.5)
 
 
+@pytest.mark.parametrize("cols", [256, 511, 512, 777, 1000, 1160, 2047, 2049, 4096, 4099, 5120, 6001,
+                                  8191, 8192, 9999, 12296, 16384])
+def test_many_rows(cols, dtype):
+    """Enough rows for every group of the streaming kernel to go round its ring, with
+    a last row that ends inside a vector where the length is odd."""
+    size = 4 if dtype == "float32" else 2
+    rows = 2 * (3 << 20) // (cols * size) | 1
+    d = make((rows, cols), dtype, (cols,), seed=cols)
+    out, h = check(d, dtype, alpha=0.75)
+    again, h2 = check({k: v[-5:] if v.ndim == 2 else v for k, v in d.items()}, dtype, alpha=0.75)
+    for a, b in ((out[-5:], again), (h[-5:], h2)):  # two orders of the sums
+        assert (a.double() - b.double()).abs().max() <= 2.0 ** -6 * b.double().abs().max()
+
+
+@pytest.mark.parametrize("cols", [1024, 1029])
+@pytest.mark.parametrize("gate", ["none", "row", "group", "full"])
+def test_many_rows_gates(gate, cols, dtype):
+    B, S = 7, 300
+    shape = {"none": None, "row": (B, S, 1), "group": (B, 1, cols), "full": (B, S, cols)}[gate]
+    check(make((B, S, cols), dtype, shape, seed=cols), dtype, alpha=1.5)
+
+
 GATES = [None, (48,), (1,), (1, 1, 48), (4, 1, 48), (4, 5, 1), (4, 1, 1), (4, 5, 48)]
 
 
