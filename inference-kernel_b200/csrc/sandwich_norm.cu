@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
   const int64_t off = (live ? row : 0) * static_cast<int64_t>(a.cols);
   const int skip = kShift ? static_cast<int>(off & (E - 1)) : 0;
   const int nv = live ? (skip + a.cols + E - 1) / E : 0;
-  const int64_t gate_at = live ? row / a.gate.rows_per * a.gate.row_stride : 0;
+  const int64_t gate_at =
+      live && gate != nullptr ? row / a.gate.rows_per * a.gate.row_stride : 0;
   const float g_row = gate != nullptr && !gate_cols ? Elem<T>::to_f(gate[gate_at]) : 1.f;
 
   auto column = [&](int i) { return (t + i * TPR) * E - skip; };  // of element 0
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   // as x and the residual), and so does the gate until its row changes.
   uint4 post[VPT], pre[VPT], g[VPT];
   float g_row = 1.f;
-  int64_t g_at = -1;
+  int64_t g_at = 0, g_end = 0;  // the gate row in use, the first row beyond it
   if constexpr (kShift) {
     keep_weight(kept, a.post, a.cols, kRingThreads);
     keep_weight(kept + room, a.pre, a.cols, kRingThreads);
@@ -502,13 +503,13 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         st_stream(reinterpret_cast<uint4*>(p + off + c), v);
     };
     if (gate != nullptr) {
-      const int64_t at = row / a.gate.rows_per;
-      if (at != g_at) {
-        g_at = at;
+      if (row >= g_end) {  // the next gate row (a division only here)
+        g_at = row / a.gate.rows_per;
+        g_end = (g_at + 1) * a.gate.rows_per;
         if (!gate_cols) {
-          g_row = Elem<T>::to_f(gate[at * a.gate.row_stride]);
+          g_row = Elem<T>::to_f(gate[g_at * a.gate.row_stride]);
         } else if constexpr (!kShift) {
-          const T* gr = gate + at * a.gate.row_stride;
+          const T* gr = gate + g_at * a.gate.row_stride;
 #pragma unroll
           for (int i = 0; i < VPT; ++i) {
             const int c = (t + i * TPR) * E;
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
 #pragma unroll
           for (int i = 0; i < VPT; ++i)
             if (used(i))
-              g[i] = load_shifted(gate, at * a.cols + column(i), a.gate.total, first(column(i)),
+              g[i] = load_shifted(gate, g_at * a.cols + column(i), a.gate.total, first(column(i)),
                                   last(column(i)));
         }
       }
