@@ -472,6 +472,17 @@ __device__ __forceinline__ void cluster_sync() {
                    : "memory");
 }
 
+// Without release semantics: for what needs none, such as mbarriers that
+// fence_mbar_init has published.  A release waits for the thread's memory
+// operations, which takes microseconds while the chip streams.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Address of the same shared-memory offset in CTA `rank` of this cluster.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
   uint32_t r;
@@ -486,6 +497,17 @@ __device__ __forceinline__ float4 ld_dsmem_f32x4(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
+}
+
+// Stores 16 bytes to a CTA of the cluster (`addr` and `bar` from map_to_rank, of
+// the same CTA) and counts them on that CTA's mbarrier when they have arrived.
+__device__ __forceinline__ void st_async_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                            uint32_t d, uint32_t bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+          addr),
+      "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
+      : "memory");
 }
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,

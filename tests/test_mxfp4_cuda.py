@@ -165,6 +165,11 @@ GEMM_SHAPES = [
     (31, 384, 14336), (32, 512, 160), (48, 4096, 1024), (64, 640, 512), (65, 129, 288),
     (128, 1024, 2048), (129, 256, 256), (130, 100, 1056), (256, 512, 1024), (257, 257, 544),
     (384, 1280, 768), (777, 1001, 1376), (1024, 2048, 512),
+    # more strips of 128 columns than clusters: several strips per cluster (M <= 32), one
+    # CTA per strip, more strips than fit at once
+    (3, 20001, 1056), (1, 24576, 2048), (20, 28700, 512), (70, 20000, 512), (2, 38001, 256),
+    # several rounds of every tile width
+    (1300, 5121, 320), (2100, 4352, 256), (700, 3584, 288), (192, 30000, 96),
 ]
 
 
