@@ -488,6 +488,29 @@ int dispatch(void* c, const void* a, const void* as, const void* b, const void* 
   return launch_tiles<T, 1, 64, 7>(c, a, as, b, bs, M, N, K, s, info);
 }
 
+// Whether M <= 128 rows go to the kernel that splits K and streams the weight at two
+// CTAs per SM (gemm_mxfp4_skinny.cu) or to one-CTA tiles.  The former's exchange of
+// partial sums grows with M, the latter go through K one block after the other; up
+// to 32 rows the former always won.  Estimates in us from graph replays on 148 SMs,
+// weight from HBM (split / 64-column tiles / 128-column tiles measured): 128 rows,
+// N x K = 6144 x 4096 12.3 / 7.1 / 7.8, 4096 x 14336 13.2 / 15.4 / 17.4, 8192 x 8192
+// 14.3 / 10.9 / 12.2, 1024 x 8192 8.2 / 10.0 / 11.1, 28672 x 4096 17.2 / 20.0 / 15.9;
+// 64 rows, 6144 x 4096 8.6 / 6.9 / 7.5, 28672 x 4096 14.5 / 19.0 / 15.0.
+bool prefer_split(int M, int N, int K, const DeviceInfo& info) {
+  if (M <= 32) return true;
+  const double weight_kb = static_cast<double>(N) * K * (17.0 / 32) / 1024;
+  const int kblocks = (K - 1) / kBK + 1;
+  auto tiles = [&](int bn, double per_block) {
+    const int64_t rounds = (tile_count(1, bn, M, N) + info.sm_count - 1) / info.sm_count;
+    const double loop = per_block * kblocks * static_cast<double>(rounds);
+    const double stream = weight_kb / 5100;
+    return 3.8 + (loop > stream ? loop : stream);
+  };
+  const double t64 = tiles(64, 0.207), t128 = tiles(128, 0.241);
+  const double split = 2.5 + 0.039 * M + weight_kb / 4900;
+  return split <= t64 && split <= t128;
+}
+
 }  // namespace
 
 int mxfp4_watchdog(uint32_t* status, bool clear) {
@@ -533,7 +556,7 @@ extern "C" int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, con
   if (int st = current_device_info(&info)) return st;
   if (int st = require_sm100(info)) return st;
   const int m = (int)M, n = (int)N, k = (int)K;
-  if (M <= kSkinnyMaxM)
+  if (M <= kSkinnyMaxM && prefer_split(m, n, k, info))
     return gemm_mxfp4_skinny(c, a, a_scales, b, b_scales, m, n, k, out_dtype, stream, info);
   switch (out_dtype) {
     case AOTK_FLOAT32: return dispatch<float>(c, a, a_scales, b, b_scales, m, n, k, s, info);
