@@ -78,6 +78,27 @@ __device__ __forceinline__ uint4 gather(const T* base, int64_t pos, int lo, int 
   return Elem<T>::pack(f);
 }
 
+// Bits of a vector's elements [lo, hi).
+template <typename T>
+__device__ __forceinline__ uint4 element_mask(int lo, int hi) {
+  constexpr int E = Elem<T>::kPerVec;
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (E == 4) {
+      w[k] = k >= lo && k < hi ? 0xFFFFFFFFu : 0u;
+    } else {
+      w[k] = (2 * k >= lo && 2 * k < hi ? 0x0000FFFFu : 0u) |
+             (2 * k + 1 >= lo && 2 * k + 1 < hi ? 0xFFFF0000u : 0u);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 operator&(const uint4& a, const uint4& b) {
+  return make_uint4(a.x & b.x, a.y & b.y, a.z & b.z, a.w & b.w);
+}
+
 // Elements [shift, shift + E) of the vectors a and b.
 template <typename T>
 __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int shift) {
@@ -133,36 +154,33 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
-// Elements of a weight kept in shared memory: whole vectors, one before and one behind.
+// A weight [cols], which starts on 16 bytes, at the places of a row that starts at
+// element `skip` of its first vector.  The weight's own last vector, if it is not
+// whole, is gathered once.
 template <typename T>
-__host__ __device__ constexpr int kept_elements(int cols) {
-  constexpr int E = Elem<T>::kPerVec;
-  return (cols + E - 1) / E * E + 2 * E;
-}
-
-// Copies a weight [cols], which starts on 16 bytes, to `kept` behind one vector of
-// zeros, zeros behind it.  All threads; the caller synchronises.
-template <typename T>
-__device__ __forceinline__ void keep_weight(T* kept, const T* w, int cols, int threads) {
-  constexpr int E = Elem<T>::kPerVec;
-  const int full = cols / E;
-  for (int v = threadIdx.x; v < full; v += threads)
-    reinterpret_cast<uint4*>(kept)[1 + v] = ld_cached(reinterpret_cast<const uint4*>(w) + v);
-  if (threadIdx.x == 0) reinterpret_cast<uint4*>(kept)[0] = make_uint4(0u, 0u, 0u, 0u);
-  const int c = full * E + threadIdx.x;
-  if (threadIdx.x < kept_elements<T>(cols) - E - full * E)
-    kept[E + c] = c < cols ? w[c] : Elem<T>::from_f(0.f);
-}
+struct ShiftedWeight {
+  static constexpr int E = Elem<T>::kPerVec;
+  const T* w;
+  int full, skip;
+  uint4 tail;
+  __device__ __forceinline__ ShiftedWeight(const T* weight, int cols, int skip_)
+      : w(weight), full(cols / E), skip(skip_), tail(gather(weight, cols / E * E, 0, cols % E)) {}
+  __device__ __forceinline__ uint4 vec(int v) const {
+    if (v >= 0 && v < full) return ld_cached(reinterpret_cast<const uint4*>(w) + v);
+    return v == full ? tail : make_uint4(0u, 0u, 0u, 0u);
+  }
+  // For vector j of the row: elements j E - skip on.
+  __device__ __forceinline__ uint4 at(int j) const {
+    return skip ? shifted<T>(vec(j - 1), vec(j), E - skip) : vec(j);
+  }
+};
 
 constexpr int threads_for(int tpr) { return tpr > 256 ? tpr : 256; }
 
 // kShift: rows need not start on 16 bytes (the tensors do).  A thread's vectors
 // are those of the tensors, so the row's first and last may hold elements of its
 // neighbours, which count as zeros and are not written; the weights' elements are
-// shifted into the places of the row's.  They are read from shared memory, where
-// each block keeps them with a vector to spare at both ends (from global memory
-// the vectors at a row's end would have to be taken apart: 127 us against 45 for
-// 20000 x 1001 bf16), and blocks go on to further rows.
+// shifted into the places of the row's.
 template <typename T, bool kShift, int VPT, int TPR>
 __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T> a) {
   constexpr int E = Elem<T>::kPerVec;
@@ -172,31 +190,18 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
   // With 1024 threads the registers hold the row, but not its weights too.
   constexpr bool kEarly = TPR < 1024;
   __shared__ float buf[2][kThreads / 32];
-  extern __shared__ __align__(16) uint8_t spare[];  // kShift: post, pre, one gate row
   const int t = threadIdx.x % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
+  const bool live = row < a.rows;
+  const int64_t off = (live ? row : 0) * static_cast<int64_t>(a.cols);
   const int64_t total = a.rows * static_cast<int64_t>(a.cols);
+  const int skip = kShift ? static_cast<int>(off & (E - 1)) : 0;
+  const int nv = live ? (skip + a.cols + E - 1) / E : 0;
   const T* gate = static_cast<const T*>(a.gate.ptr);
   const bool gate_cols = gate != nullptr && a.gate.col_stride;
-  const bool gate_kept = kShift && gate_cols && a.gate.total == a.cols;
-  const int room = kept_elements<T>(a.cols);
-  T* kept = reinterpret_cast<T*>(spare);
 
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
-  if constexpr (kShift) {
-    keep_weight(kept, a.post, a.cols, kThreads);
-    keep_weight(kept + room, a.pre, a.cols, kThreads);
-    if (gate_kept) keep_weight(kept + 2 * room, gate, a.cols, kThreads);
-    __syncthreads();
-  }
-  // One pass unless kShift.
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPB; row0 < a.rows;
-       row0 += static_cast<int64_t>(gridDim.x) * RPB) {
-  const int64_t row = row0 + threadIdx.x / TPR;
-  const bool live = row < a.rows;
-  const int64_t off = (live ? row : 0) * static_cast<int64_t>(a.cols);
-  const int skip = kShift ? static_cast<int>(off & (E - 1)) : 0;
-  const int nv = live ? (skip + a.cols + E - 1) / E : 0;
   const int64_t gate_at =
       live && gate != nullptr ? row / a.gate.rows_per * a.gate.row_stride : 0;
   const float g_row = gate != nullptr && !gate_cols ? Elem<T>::to_f(gate[gate_at]) : 1.f;
@@ -210,19 +215,8 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
       if (off + c + E > total) return gather(p, off + c, first(c), last(c));
     return ld_stream(reinterpret_cast<const uint4*>(p + off + c));
   };
-  auto col_vec = [&](const T* p, int c, int which) {  // of a weight, or the only gate row
-    if constexpr (kShift) {
-      // Element c is at E + c there: the same shift for the whole row.
-      const uint4* v = reinterpret_cast<const uint4*>(kept + which * room) + (c + skip) / E;
-      return skip ? shifted<T>(v[0], v[1], E - skip) : v[1];
-    }
-    return ld_cached(reinterpret_cast<const uint4*>(p + c));
-  };
   auto gate_vec = [&](int c) {
-    if constexpr (kShift) {
-      if (gate_kept) return col_vec(gate, c, 2);
-      return load_shifted(gate, gate_at + c, a.gate.total, first(c), last(c));
-    }
+    if constexpr (kShift) return load_shifted(gate, gate_at + c, a.gate.total, first(c), last(c));
     return ld_cached(reinterpret_cast<const uint4*>(gate + gate_at + c));
   };
   auto write = [&](T* p, int c, const float2* f) {
@@ -258,11 +252,16 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
       res[i] = row_vec(a.residual, column(i));
     }
   }
+  const ShiftedWeight<T> post_w(a.post, a.cols, skip), pre_w(a.pre, a.cols, skip);
+  auto weight_vec = [&](const ShiftedWeight<T>& w, int i) {
+    if constexpr (kShift) return w.at(t + i * TPR);
+    return ld_cached(reinterpret_cast<const uint4*>(w.w) + t + i * TPR);
+  };
   auto load_post = [&](int i) {
-    post[i] = col_vec(a.post, column(i), 0);
+    post[i] = weight_vec(post_w, i);
     if (gate_cols) g[i] = gate_vec(column(i));
   };
-  auto load_pre = [&](int i) { pre[i] = col_vec(a.pre, column(i), 1); };
+  auto load_pre = [&](int i) { pre[i] = weight_vec(pre_w, i); };
   if constexpr (kEarly) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -326,8 +325,6 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
       write(a.out, column(i), w);
     }
   }
-  if constexpr (!kShift) break;
-  }
 }
 
 // ---- many rows: a ring of rows in shared memory ----------------------------------
@@ -341,11 +338,8 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
 constexpr int kRingThreads = 512;
 constexpr int kRingBytes = 196608;
 constexpr int kMaxStages = 8;
-#ifndef RTOT
-#define RTOT (1 << 20)
-#endif
-constexpr int64_t kRingMinRow = 1024, kRingMaxRow = 32768, kRingMinTotal = RTOT;
-constexpr int64_t kRingMaxShift = 16384;  // with the weights beside the ring
+constexpr int64_t kRingMinRow = 1024, kRingMinTotal = 1 << 20;  // bytes
+constexpr int64_t kRingMaxVectors = 4 * kRingThreads;           // of a row
 
 __device__ unsigned g_norm_watchdog;
 enum : unsigned { kWdRow = 262144u };
@@ -386,8 +380,9 @@ __device__ __forceinline__ void group_sync(int group) {
 
 // kShift: rows need not start on 16 bytes (the tensors do).  The copies take the
 // vectors around a row, a thread works on those, and the row's first and last are
-// written element by element; weights come from shared memory, shifted into the
-// places of the row's elements.
+// written element by element.  The grid makes a group's rows `step` apart with step
+// a multiple of E, so they all start at the same element of a vector, and weights
+// shifted to it once stay in registers like those of aligned rows.
 template <typename T, bool kShift, int VPT, int TPR>
 __global__ void __launch_bounds__(kRingThreads, 1)
     sandwich_ring_kernel(const Args<T> a, int stages, int pitch) {
@@ -396,7 +391,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   constexpr int P = E / 2;  // pairs per vector
   constexpr int G = kRingThreads / TPR;
   constexpr int WPR = TPR / 32;
-  extern __shared__ __align__(16) uint8_t ring[];  // [G][stages][x, residual][pitch], then weights
+  extern __shared__ __align__(16) uint8_t ring[];  // [G][stages][x, residual][pitch]
   __shared__ float partial[G][2][WPR];
   __shared__ __align__(8) uint64_t bars[G][kMaxStages];
   __shared__ __align__(16) uint4 ends[kShift ? G : 1][2][2];  // [h, out][first, last vector]
@@ -410,9 +405,30 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   const uint32_t bar0 = smem_addr(bars[group]);
   const T* gate = static_cast<const T*>(a.gate.ptr);
   const bool gate_cols = gate != nullptr && a.gate.col_stride;
-  const bool gate_kept = kShift && gate_cols && a.gate.total == a.cols;
-  const int room = kept_elements<T>(a.cols);
-  T* kept = reinterpret_cast<T*>(ring + static_cast<int64_t>(G) * stages * 2 * pitch);
+  // Of every row of this group (step is a multiple of E).
+  const int skip = kShift ? static_cast<int>(first_row * a.cols & (E - 1)) : 0;
+  const int nv = (skip + a.cols + E - 1) / E;
+  auto column = [&](int i) { return (t + i * TPR) * E - skip; };  // of element 0
+  auto used = [&](int i) { return t + i * TPR < nv; };
+  const int last_i = (nv - 1) / TPR;
+  uint4 head, foot;  // of the thread's vectors 0 and last_i
+  bool head_cut = false, foot_cut = false;
+  T* end_to = nullptr;
+  const T* end_from = nullptr;
+  if constexpr (kShift) {
+    const int c = column(0), d = column(last_i);
+    head = element_mask<T>(c < 0 ? -c : 0, E);
+    foot = element_mask<T>(0, a.cols - d < E ? a.cols - d : E);
+    head_cut = c < 0;
+    foot_cut = d < a.cols && d + E > a.cols;
+    // One thread per element of the shared vectors: [h, out][first, last][element].
+    const int which = t / (2 * E), end = t / E % 2, e = t % E;
+    const int at = (end ? nv - 1 : 0) * E - skip + e;
+    if (t < 4 * E && at >= 0 && at < a.cols && (end ? (nv * E - skip) > a.cols : skip > 0)) {
+      end_to = (which ? a.out : a.h_out) + at;
+      end_from = reinterpret_cast<const T*>(&ends[kShift ? group : 0][which][end]) + e;
+    }
+  }
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -445,24 +461,20 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int k = 0; k < stages && first_row + k * step < a.rows; ++k)
       request(first_row + k * step, k);
 
-  // Rows that start on 16 bytes: a thread's columns are the same in every row, so
-  // their weights stay in registers (from L2 they would be as many bytes per row
-  // as x and the residual), and so does the gate until its row changes.
+  // A thread's columns are the same in every row, so their weights stay in
+  // registers (from L2 they would be as many bytes per row as x and the residual),
+  // and so does the gate until its row changes.
   uint4 post[VPT], pre[VPT], g[VPT];
   float g_row = 1.f;
   int64_t g_at = 0, g_end = 0;  // the gate row in use, the first row beyond it
-  if constexpr (kShift) {
-    keep_weight(kept, a.post, a.cols, kRingThreads);
-    keep_weight(kept + room, a.pre, a.cols, kRingThreads);
-    if (gate_kept) keep_weight(kept + 2 * room, gate, a.cols, kRingThreads);
-    __syncthreads();
-  } else {
+  {
+    const ShiftedWeight<T> post_w(a.post, a.cols, skip), pre_w(a.pre, a.cols, skip);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = (t + i * TPR) * E;
-      if (c < a.cols) {
-        post[i] = ld_cached(reinterpret_cast<const uint4*>(a.post + c));
-        pre[i] = ld_cached(reinterpret_cast<const uint4*>(a.pre + c));
+      const int j = t + i * TPR;
+      if (j < nv) {
+        post[i] = kShift ? post_w.at(j) : ld_cached(reinterpret_cast<const uint4*>(a.post) + j);
+        pre[i] = kShift ? pre_w.at(j) : ld_cached(reinterpret_cast<const uint4*>(a.pre) + j);
       }
     }
   }
@@ -471,79 +483,67 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   uint32_t phase = 0;
   for (int64_t row = first_row; row < a.rows; row += step) {
     const int64_t off = row * a.cols;
-    const int skip = kShift ? static_cast<int>(off & (E - 1)) : 0;
-    const int nv = (skip + a.cols + E - 1) / E;
-    auto column = [&](int i) { return (t + i * TPR) * E - skip; };  // of element 0
-    auto used = [&](int i) { return t + i * TPR < nv; };
-    auto first = [&](int c) { return kShift && c < 0 ? -c : 0; };
-    auto last = [&](int c) { return kShift && a.cols - c < E ? a.cols - c : E; };
-    auto kept_vec = [&](int which, int i) {
-      const uint4* v = reinterpret_cast<const uint4*>(kept + which * room) + t + i * TPR;
-      return skip ? shifted<T>(v[0], v[1], E - skip) : v[1];
-    };
-    auto mask = [&](int c, float2* f) {  // zeros where the row is not
+    // Zeros where a vector is not the row's; only the first and the last are shared.
+    auto own = [&](const uint4& v, int i) {
       if constexpr (kShift) {
-        const int lo = first(c), hi = last(c);
-        if (lo > 0 || hi < E) {
-#pragma unroll
-          for (int k = 0; k < P; ++k) {
-            if (2 * k < lo || 2 * k >= hi) f[k].x = 0.f;
-            if (2 * k + 1 < lo || 2 * k + 1 >= hi) f[k].y = 0.f;
-          }
-        }
+        if (i == 0 && last_i == 0) return v & head & foot;
+        if (i == 0) return v & head;
+        if (i == last_i) return v & foot;
       }
+      return v;
     };
     // A whole vector goes to its place, one that the row shares to `ends`.
     auto write = [&](T* p, int which, int i, const float2* f) {
       const uint4 v = Elem<T>::pack(&f[0].x);
-      const int c = column(i);
-      if (kShift && (c < 0 || c + E > a.cols))
-        ends[kShift ? group : 0][which][c < 0 ? 0 : 1] = v;
+      if (kShift && i == 0 && head_cut)
+        ends[kShift ? group : 0][which][0] = v;
+      else if (kShift && i == last_i && foot_cut)
+        ends[kShift ? group : 0][which][1] = v;
       else
-        st_stream(reinterpret_cast<uint4*>(p + off + c), v);
+        st_stream(reinterpret_cast<uint4*>(p + off + column(i)), v);
     };
-    if (gate != nullptr) {
-      if (row >= g_end) {  // the next gate row (a division only here)
-        g_at = row / a.gate.rows_per;
-        g_end = (g_at + 1) * a.gate.rows_per;
-        if (!gate_cols) {
-          g_row = Elem<T>::to_f(gate[g_at * a.gate.row_stride]);
-        } else if constexpr (!kShift) {
-          const T* gr = gate + g_at * a.gate.row_stride;
+    if (gate != nullptr && row >= g_end) {  // the next gate row (a division only here)
+      g_at = row / a.gate.rows_per;
+      g_end = (g_at + 1) * a.gate.rows_per;
+      const int64_t at = g_at * a.gate.row_stride;
+      if (gate_cols) {
 #pragma unroll
-          for (int i = 0; i < VPT; ++i) {
-            const int c = (t + i * TPR) * E;
-            if (c < a.cols) g[i] = ld_cached(reinterpret_cast<const uint4*>(gr + c));
+        for (int i = 0; i < VPT; ++i)
+          if (used(i)) {
+            const int c = column(i);
+            if constexpr (kShift) {
+              const int left = a.cols - c;
+              g[i] = own(load_shifted(gate, at + c, a.gate.total, c < 0 ? -c : 0, left < E ? left : E), i);
+            } else {
+              g[i] = ld_cached(reinterpret_cast<const uint4*>(gate + at + c));
+            }
           }
-        }
-      }
-      if constexpr (kShift) {
-        if (gate_cols && !gate_kept) {
-#pragma unroll
-          for (int i = 0; i < VPT; ++i)
-            if (used(i))
-              g[i] = load_shifted(gate, g_at * a.cols + column(i), a.gate.total, first(column(i)),
-                                  last(column(i)));
-        }
+      } else {
+        g_row = Elem<T>::to_f(gate[at]);
       }
     }
     const uint4* xs = reinterpret_cast<const uint4*>(mine + static_cast<int64_t>(stage) * 2 * pitch);
     const uint4* rs = reinterpret_cast<const uint4*>(mine + (static_cast<int64_t>(stage) * 2 + 1) * pitch);
-    // The tensor's last elements may lie behind its last whole vector.
-    const bool cut = kShift && off + a.cols == total && total % E != 0;
-    auto row_vec = [&](const uint4* sm, const T* gm, int i) {
-      if (cut && t + i * TPR == nv - 1) return gather(gm, off + column(i), first(column(i)), last(column(i)));
-      return sm[t + i * TPR];
-    };
     bool bad = !mbar_wait_bounded(bar0 + 8u * stage, phase, &abort_flag, &g_norm_watchdog, kWdRow);
+    if constexpr (kShift) {
+      // The tensor's last elements, if they lie behind its last whole vector.
+      const int rest = static_cast<int>(total & (E - 1));
+      if (rest > 0 && off + a.cols == total) {
+        if (t < rest) {
+          uint8_t* at = mine + static_cast<int64_t>(stage) * 2 * pitch + ((nv - 1) * E + t) * sizeof(T);
+          *reinterpret_cast<T*>(at) = a.x[total - rest + t];
+          *reinterpret_cast<T*>(at + pitch) = a.residual[total - rest + t];
+        }
+        group_sync<TPR>(group);
+      }
+    }
 
     float2 h[VPT][P];  // x, then h
     float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
-        Elem<T>::unpack(row_vec(xs, a.x, i), &h[i][0].x);
-        mask(column(i), h[i]);
+        Elem<T>::unpack(own(xs[t + i * TPR], i), &h[i][0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) ss = fma2(h[i][e], h[i][e], ss);
       }
@@ -559,20 +559,20 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(kShift ? kept_vec(0, i) : post[i], &w[0].x);
+        Elem<T>::unpack(post[i], &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) h[i][e] = mul2(mul2(h[i][e], scale2), w[e]);
         if (gate_cols) {
-          Elem<T>::unpack(gate_kept ? kept_vec(2, i) : g[i], &w[0].x);
+          Elem<T>::unpack(g[i], &w[0].x);
 #pragma unroll
           for (int e = 0; e < P; ++e) h[i][e] = mul2(h[i][e], w[e]);
         }
-        Elem<T>::unpack(row_vec(rs, a.residual, i), &w[0].x);
+        Elem<T>::unpack(own(rs[t + i * TPR], i), &w[0].x);
 #pragma unroll
-        for (int e = 0; e < P; ++e) h[i][e] = fma2(alpha2, w[e], h[i][e]);
-        mask(column(i), h[i]);
-#pragma unroll
-        for (int e = 0; e < P; ++e) ss = fma2(h[i][e], h[i][e], ss);
+        for (int e = 0; e < P; ++e) {
+          h[i][e] = fma2(alpha2, w[e], h[i][e]);
+          ss = fma2(h[i][e], h[i][e], ss);
+        }
         write(a.h_out, 0, i, h[i]);
       }
     }
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(kShift ? kept_vec(1, i) : pre[i], &w[0].x);
+        Elem<T>::unpack(pre[i], &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) w[e] = mul2(mul2(h[i][e], inv_h2), w[e]);
         write(a.out, 1, i, w);
@@ -594,13 +594,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     if constexpr (kShift) {
       // One lane per element of the first and the last vector, if they are shared.
       group_sync<TPR>(group);
-      if (t < 4 * E) {
-        const int which = t / (2 * E), end = t / E % 2, e = t % E;
-        const int c = (end ? nv - 1 : 0) * E - skip;
-        if ((end ? c + E > a.cols : c < 0) && c + e >= 0 && c + e < a.cols)
-          (which ? a.out : a.h_out)[off + c + e] =
-              reinterpret_cast<const T*>(&ends[kShift ? group : 0][which][end])[e];
-      }
+      if (end_to != nullptr) end_to[off] = *end_from;
       group_sync<TPR>(group);
     }
     if (++stage == stages) {
@@ -687,13 +681,12 @@ __global__ void __launch_bounds__(kLongThreads) sandwich_long_kernel(const Args<
 
 template <typename T>
 int launch_kernel(void (*kernel)(const Args<T>), const Args<T>& a, int64_t blocks, int threads,
-                  size_t smem, cudaStream_t s) {
+                  cudaStream_t s) {
   if (blocks > 0x7fffffffLL)
     return fail(AOTK_ERR_INVALID_ARGUMENT, "aotk_sandwich_rmsnorm: too many rows");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -709,27 +702,13 @@ int launch_kernel(void (*kernel)(const Args<T>), const Args<T>& a, int64_t block
 template <typename T, bool kShift, int VPT, int TPR>
 int launch_rows(const Args<T>& a, cudaStream_t s) {
   constexpr int kThreads = threads_for(TPR);
-  auto kernel = sandwich_kernel<T, kShift, VPT, TPR>;
-  int64_t blocks = (a.rows + kThreads / TPR - 1) / (kThreads / TPR);
-  size_t smem = 0;
-  if constexpr (kShift) {
-    DeviceInfo info;
-    if (int st = current_device_info(&info)) return st;
-    smem = 3 * sizeof(T) * static_cast<size_t>(kept_elements<T>(a.cols));
-    // The largest room this kernel may need: VPT * TPR vectors of a row.
-    constexpr size_t most = 3 * 16 * (static_cast<size_t>(VPT) * TPR + 2);
-    if (most > 48 * 1024)
-      if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), most, info)) return st;
-    const int64_t resident = static_cast<int64_t>(info.sm_count) *
-                             (kThreads > 256 || smem > 100 * 1024 ? 1 : smem > 64 * 1024 ? 2 : 3);
-    if (blocks > resident) blocks = resident;
-  }
-  return launch_kernel<T>(kernel, a, blocks, kThreads, smem, s);
+  const int64_t blocks = (a.rows + kThreads / TPR - 1) / (kThreads / TPR);
+  return launch_kernel<T>(sandwich_kernel<T, kShift, VPT, TPR>, a, blocks, kThreads, s);
 }
 
 template <typename T, int E>
 int launch_long(const Args<T>& a, cudaStream_t s) {
-  return launch_kernel<T>(sandwich_long_kernel<T, E>, a, a.rows, kLongThreads, 0, s);
+  return launch_kernel<T>(sandwich_long_kernel<T, E>, a, a.rows, kLongThreads, s);
 }
 
 // The smallest group of threads that holds a row in at most four vectors each.
@@ -755,16 +734,20 @@ int launch_ring(const Args<T>& a, cudaStream_t s, const DeviceInfo& info) {
   constexpr int G = kRingThreads / TPR;
   constexpr int E = Elem<T>::kPerVec;
   const int pitch = ((a.cols + E - 1) / E + (kShift ? 1 : 0)) * 16;
-  const int weights = kShift ? 3 * static_cast<int>(sizeof(T)) * kept_elements<T>(a.cols) : 0;
-  int stages = (kRingBytes - weights) / (G * 2 * pitch);
+  int stages = kRingBytes / (G * 2 * pitch);
   if (stages > kMaxStages) stages = kMaxStages;
   auto kernel = sandwich_ring_kernel<T, kShift, VPT, TPR>;
   if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes, info)) return st;
-  const int64_t groups = (a.rows + G - 1) / G;
+  int64_t blocks = (a.rows + G - 1) / G;
+  if (blocks > info.sm_count) {
+    // Groups that take several rows: blocks x G, the rows between them, a multiple of E.
+    constexpr int unit = E > G ? E / G : 1;
+    blocks = kShift ? info.sm_count / unit * unit : info.sm_count;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(groups < info.sm_count ? groups : info.sm_count), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
   cfg.blockDim = dim3(kRingThreads, 1, 1);
-  cfg.dynamicSmemBytes = static_cast<size_t>(G) * stages * 2 * pitch + weights;
+  cfg.dynamicSmemBytes = static_cast<size_t>(G) * stages * 2 * pitch;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -813,8 +796,8 @@ int launch(void* out, void* h_out, const void* x, const void* residual, const vo
   if (int st = current_device_info(&info)) return st;
   const bool shift = cols % E != 0;
   const int64_t row_bytes = cols * static_cast<int64_t>(sizeof(T));
-  if (row_bytes >= kRingMinRow && row_bytes <= (shift ? kRingMaxShift : kRingMaxRow) &&
-      rows * row_bytes >= kRingMinTotal)
+  const int64_t vectors = (cols + (shift ? 2 * (E - 1) : 0)) / E;
+  if (row_bytes >= kRingMinRow && vectors <= kRingMaxVectors && rows * row_bytes >= kRingMinTotal)
     return shift ? dispatch_ring<T, true>(a, s, info) : dispatch_ring<T, false>(a, s, info);
   return shift ? dispatch_rows<T, true>(a, s) : dispatch_rows<T, false>(a, s);
 }

@@ -72,7 +72,7 @@ def test_row_counts(rows, dtype):
 
 
 @pytest.mark.parametrize("cols", [256, 511, 512, 777, 1000, 1160, 2047, 2049, 4096, 4099, 5120, 6001,
-                                  8191, 8192, 9999, 12296, 16384])
+                                  8189, 8191, 8192, 9999, 12296, 16371, 16383, 16384])
 def test_many_rows(cols, dtype):
     """Enough rows for every group of the streaming kernel to go round its ring, with
     a last row that ends inside a vector where the length is odd."""
