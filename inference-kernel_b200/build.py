@@ -124,6 +124,7 @@ def build_torch_ext(verbose: bool = False) -> Path:
         "-lc10",
         "-lc10_cuda",
         "-ltorch_cpu",
+        "-ltorch_cuda",
         "-ltorch",
         "-Wl,-rpath,$ORIGIN",
         f"-Wl,-rpath,{torch_lib}",

@@ -354,6 +354,60 @@ def test_side_stream_and_graph(M):
         assert all(torch.equal(p, q) for p, q in zip(got, want[i]))
 
 
+def test_two_streams_at_once():
+    """Products of every kernel on two streams, many in flight, against one alone."""
+    import torch
+
+    import aot_kernel
+
+    K = 1024
+    work = []
+    for j, (M, N) in enumerate(((1, 2048), (40, 4096), (120, 640), (300, 2048), (1000, 1500))):
+        a = aot_kernel.mxfp4_quantize(to_device(randn((M, K), j), "bfloat16"))
+        b = aot_kernel.mxfp4_quantize(to_device(randn((N, K), 50 + j), "bfloat16"))
+        work.append((a, b, aot_kernel.mxfp4_gemm(*a, *b)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for r in range(6):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for a, b, want in work[:: 1 - 2 * k]:
+                    got.append((aot_kernel.mxfp4_gemm(*a, *b), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in got)
+    from aot_kernel import capi
+
+    assert capi.watchdog_status() == 0
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in x, in the values read back and in the product."""
+    import torch
+
+    import aot_kernel
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rows, cols = 65700, 32768
+    x = torch.randn(rows, cols, generator=gen, device="cuda", dtype=torch.bfloat16)
+    codes, scales = aot_kernel.mxfp4_quantize(x)
+    back = aot_kernel.mxfp4_dequantize(codes, scales)
+    for r0 in (0, 65536 - 128, 65536 + 128 - 128):
+        part = x[r0:r0 + 128].contiguous()
+        c, s = aot_kernel.mxfp4_quantize(part)
+        assert torch.equal(codes[r0:r0 + 128], c) and torch.equal(scales[r0 // 128], s[0])
+        assert torch.equal(back[r0:r0 + 128], aot_kernel.mxfp4_dequantize(c, s))
+    del x, back, codes, scales
+    M, N, K = 65700, 32896, 64
+    a = aot_kernel.mxfp4_quantize(torch.randn(M, K, generator=gen, device="cuda"))
+    b = aot_kernel.mxfp4_quantize(torch.randn(N, K, generator=gen, device="cuda"))
+    out = aot_kernel.mxfp4_gemm(*a, *b)
+    av, bv = (aot_kernel.mxfp4_dequantize(*q, torch.float32) for q in (a, b))
+    for r0 in (0, 65600):  # sums of 64 products of a few bits each: exact in fp32
+        want = (av[r0:r0 + 64].double() @ bv.double().t()).float().to(torch.bfloat16)
+        assert torch.equal(out[r0:r0 + 64], want)
+
+
 @pytest.mark.parametrize("M", [1, 9, 260])
 def test_block_in_four_bits(M):
     """One gated MLP block served in 4 bits between its norms: quantise, gate/up

@@ -257,3 +257,24 @@ def test_stream_and_graph():
     new = step()
     assert all(torch.equal(a, b) for a, b in zip(got, new))
     assert not torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("cols", [16384, 8191])
+def test_offsets_beyond_32_bits(cols):
+    import torch
+
+    import aot_kernel
+
+    rows = (1 << 31) // cols + 300
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(rows, cols, generator=gen, device="cuda", dtype=torch.bfloat16)
+    residual = torch.randn(rows, cols, generator=gen, device="cuda", dtype=torch.bfloat16)
+    post, pre = (torch.randn(cols, generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    gate = torch.randn(rows, 1, generator=gen, device="cuda", dtype=torch.bfloat16)
+    out, h = aot_kernel.sandwich_rmsnorm(x, residual, post, pre, EPS, gate=gate)
+    for r0 in (0, rows - 9):
+        part = [t[r0:r0 + 9].clone() for t in (x, residual, gate)]
+        o, hh = aot_kernel.sandwich_rmsnorm(part[0], part[1], post, pre, EPS, gate=part[2])
+        for g, w in ((out, o), (h, hh)):  # sums in another order: at most one step of bf16
+            g = g[r0:r0 + 9].double()
+            assert ((g - w.double()).abs() <= 2.0 ** -7 * w.double().abs() + 1e-3).all()
