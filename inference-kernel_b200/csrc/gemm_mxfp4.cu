@@ -16,7 +16,11 @@
 //     holds the stage barriers and issues all MMAs; each reads out its 128 rows;
 //   * 8 epilogue warps read a tile out of TMEM at once, 128 columns each at
 //     BN = 256, so one accumulator is enough there (it and the scales would not
-//     fit twice into 512 columns); narrower tiles have two.
+//     fit twice into 512 columns); narrower tiles have two.  A lane holds a row and
+//     writes it in whole 32-byte sectors, without shared memory, which is the
+//     ring's (staged TMA stores and a stage less: 8192^3 226 -> 232 us, 128 x 6144 x
+//     4096 7.0 -> 7.1).  Where rows do not start on 16 bytes, the memory of two
+//     stages turns the rows for stores along them.
 // What bounds it: tiles of one CTA by operand traffic out of L2, about 16.5 TB/s
 // over the chip (128 x 256 tiles: 51 KB per 256 of K, 0.455 us where the MMAs take
 // 0.27); pairs of CTAs move 35 KB for the same work and end at the power cap.
@@ -58,9 +62,11 @@ struct MxLayout {
   static constexpr uint32_t kOffA = 0;
   static constexpr uint32_t kOffB = kOffA + STAGES * kABytes;
   static constexpr uint32_t kOffSf = kOffB + STAGES * kBBytes;
+  static constexpr uint32_t kOffBar = kOffSf + STAGES * kSfBytes;
+  // Staging of unaligned rows: 4 KB per epilogue warp in A's last two stages.
   static constexpr uint32_t kCBuf = 32 * 128;
-  static constexpr uint32_t kOffC = kOffSf + STAGES * kSfBytes;
-  static constexpr uint32_t kOffBar = kOffC + kEpiWarps * kCBuf;
+  static constexpr uint32_t kOffC = kOffA + (STAGES - 2) * kABytes;
+  static_assert(kEpiWarps * kCBuf <= 2 * kABytes, "staging fits two stages");
   static constexpr uint32_t kNumBars = 2 * STAGES + 5;  // full, empty, tfull x2, release x2, drain
   static constexpr uint32_t kOffMisc = kOffBar + kNumBars * 8;
   static constexpr uint32_t kAlloc = kOffMisc + 16 + 1024;
@@ -93,43 +99,60 @@ __device__ __forceinline__ uint32_t pack_word(const uint32_t* r, int i) {
     return Elem<T>::pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 
-// Writes a warp's 32 rows x 128 bytes of accumulators (lane = row) to C at (x, y)
-// through its 4 KB staging buffer: a TMA store, or element stores a row at a
-// time where a row stride or the base is not a multiple of 16 bytes.
+enum : int { kRowsAny = 0, kRows16 = 1, kRows32 = 2 };  // bytes that rows of C start on
+
+// Writes a warp's 32 rows x 128 bytes of accumulators (lane = row) to C at (x, y).
+// A lane writes its row's vectors; rows that do not start on 16 bytes are turned
+// through 4 KB of shared memory and written element by element along the row.
 template <typename T>
-__device__ __forceinline__ void store_chunk(const CUtensorMap* tmC, T* __restrict__ c,
-                                            const uint32_t* r, uint32_t buf, const uint8_t* buf_ptr,
-                                            int lane, int x, int y, int M, int N, int tma_store) {
+__device__ __forceinline__ void store_chunk(T* __restrict__ c, const uint32_t* r, uint8_t* buf,
+                                            int lane, int x, int y, int M, int N, int rows_on) {
   constexpr int kChunk = 128 / sizeof(T);
-  if (tma_store && lane == 0) bulk_wait_read<0>();
-  __syncwarp();
-  const uint32_t srow = buf + lane * 128;
+  constexpr int kVec = 16 / sizeof(T);
+  auto vec = [&](int j) {
+    return make_uint4(pack_word<T>(r, 4 * j), pack_word<T>(r, 4 * j + 1), pack_word<T>(r, 4 * j + 2),
+                      pack_word<T>(r, 4 * j + 3));
+  };
+  if (rows_on != kRowsAny) {
+    if (y + lane >= M) return;
+    T* p = c + static_cast<int64_t>(y + lane) * N + x;
+    auto one = [&](int j) {
+      if (x + j * kVec < N) st_stream(reinterpret_cast<uint4*>(p + j * kVec), vec(j));
+    };
+    auto two = [&](int j) {
+      if (x + (j + 1) * kVec < N)
+        st_stream32(p + j * kVec, vec(j), vec(j + 1));
+      else
+        one(j);
+    };
+    // Whole sectors also where every other row starts in the middle of one.
+    if (rows_on == kRows32 || reinterpret_cast<uintptr_t>(p) % 32 == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) two(j);
+    } else {
+      one(0);
+#pragma unroll
+      for (int j = 1; j < 7; j += 2) two(j);
+      one(7);
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    st_shared_v4(srow + ((j ^ (lane & 7)) << 4), pack_word<T>(r, 4 * j), pack_word<T>(r, 4 * j + 1),
-                 pack_word<T>(r, 4 * j + 2), pack_word<T>(r, 4 * j + 3));
-  if (tma_store) {
-    fence_proxy_async_shared();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_2d(tmC, buf, x, y);
-      bulk_commit();
-    }
-  } else {
-    __syncwarp();
-    const int rows = min(32, M - y);
-    for (int rr = 0; rr < rows; ++rr) {
-      T* crow = c + static_cast<int64_t>(y + rr) * N + x;
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = vec(j);
+  __syncwarp();
+  const int rows = min(32, M - y);
+  for (int rr = 0; rr < rows; ++rr) {
+    T* crow = c + static_cast<int64_t>(y + rr) * N + x;
 #pragma unroll
-      for (int e = lane; e < kChunk; e += 32) {
-        const int b = e * static_cast<int>(sizeof(T));
-        const T v = *reinterpret_cast<const T*>(buf_ptr + rr * 128 + (((b >> 4) ^ (rr & 7)) << 4) +
-                                                (b & 15));
-        if (x + e < N) crow[e] = v;
-      }
+    for (int e = lane; e < kChunk; e += 32) {
+      const int b = e * static_cast<int>(sizeof(T));
+      const T v =
+          *reinterpret_cast<const T*>(buf + rr * 128 + (((b >> 4) ^ (rr & 7)) << 4) + (b & 15));
+      if (x + e < N) crow[e] = v;
     }
-    __syncwarp();
   }
+  __syncwarp();
 }
 
 template <typename T, int CG, int BN, int STAGES>
@@ -137,13 +160,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
                       const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmSa,
-                      const __grid_constant__ CUtensorMap tmSb,
-                      const __grid_constant__ CUtensorMap tmC, T* __restrict__ c, int M, int N,
-                      int K, int tma_store) {
+                      const __grid_constant__ CUtensorMap tmSb, T* __restrict__ c, int M, int N,
+                      int K, int rows_on) {
   using L = MxLayout<CG, BN, STAGES>;
   constexpr int kTileM = CG * kBM;
   constexpr int kGroup = kGroupRows / kTileM;
-  constexpr int kChunk = 128 / sizeof(T);                // output columns per staged box
+  constexpr int kChunk = 128 / sizeof(T);                // columns of 128 bytes of output
   constexpr int kHalves = BN / 2 >= kChunk ? 2 : 1;      // warps that share a row's columns
   constexpr int kRead = BN / kHalves;                    // columns read by a warp
   extern __shared__ uint8_t smem_raw[];
@@ -170,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int num_tiles = tiles_m * tiles_n;
   const int kblocks = (K + kBK - 1) / kBK;
   const int sf_tiles_k = (K + 127) / 128;
+  const int stages = rows_on == kRowsAny ? STAGES - 2 : STAGES;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -200,7 +223,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();  // both CTAs' barriers before any use across
+  if constexpr (CG == 2) {  // both CTAs' barriers before any use across
+    cluster_arrive_relaxed();
+    cluster_wait();
+  }
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // Global memory is touched only from here on, once the previous kernel on
@@ -252,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         ++issued;
-        if (++stage == STAGES) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -262,9 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elected && rank == 0) {
       int s = stage;
       uint32_t p = phase;
-      for (int i = 0; i < STAGES && i < issued; ++i) {
+      for (int i = 0; i < stages && i < issued; ++i) {
         if (--s < 0) {
-          s = STAGES - 1;
+          s = stages - 1;
           p ^= 1u;
         }
         mbar_drain(full_bar(s), p);
@@ -341,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             commit(empty_bar(stage));
           }
           __syncwarp();
-          if (++stage == STAGES) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -360,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- epilogue (every CTA) ----------------
     const int q = warp & 3;            // the quarter of TMEM lanes that this warp may read
     const int half = (warp - 2) / 4;   // its columns of the tile
-    const uint32_t off = L::kOffC + (warp - 2) * L::kCBuf;
+    uint8_t* buf = smem + L::kOffC + (warp - 2) * L::kCBuf;
     int it = 0;
     for (int tile = worker; tile < num_tiles; tile += workers, ++it) {
       int mb, nb;
@@ -391,20 +417,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < kRead / kChunk; ++j) {
         const int x = nb * BN + half * kRead + j * kChunk;
         if (x < N && y < M)
-          store_chunk<T>(&tmC, c, r + j * kChunk, base + off, smem + off, lane, x, y, M, N,
-                         tma_store);
+          store_chunk<T>(c, r + j * kChunk, buf, lane, x, y, M, N, rows_on);
       }
     }
-    // The buffers have been read; the writes are done when the kernel is.
-    if (lane == 0) bulk_wait_read<0>();
-    __syncwarp();
   }
 
   // No CTA frees TMEM or exits while its pair may still use its shared memory
   // (operands, barriers) or its TMEM.
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
+  if constexpr (CG == 2) {
+    cluster_arrive_relaxed();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after();
     if constexpr (CG == 2)
@@ -412,16 +437,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     else
       tmem_dealloc(tmem_base, L::kTmemCols);
   }
-}
-
-template <typename T>
-int output_map(CUtensorMap* tm, const void* c, int M, int N, int* tma_store) {
-  *tma_store = aligned16(c) && static_cast<int64_t>(N) * sizeof(T) % 16 == 0;
-  if (!*tma_store) return AOTK_OK;
-  if constexpr (std::is_same_v<T, float>)
-    return make_tmap_2d_f32(tm, c, M, N, N, 32, 32);
-  else
-    return make_tmap_2d_16bit(tm, c, std::is_same_v<T, __nv_bfloat16>, M, N, N, 64, 32);
 }
 
 int64_t tile_count(int cg, int bn, int M, int N) {
@@ -434,8 +449,7 @@ int launch_tiles(void* c, const void* a, const void* as, const void* b, const vo
   using L = MxLayout<CG, BN, STAGES>;
   auto kernel = gemm_mxfp4_kernel<T, CG, BN, STAGES>;
   if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, info)) return st;
-  CUtensorMap ta, tb, tsa, tsb, tc = {};
-  int tma_store = 0;
+  CUtensorMap ta, tb, tsa, tsb;
   const uint64_t sf_tiles_k = (static_cast<uint64_t>(K) + 127) / 128;
   if (int st = make_tmap_2d_8bit(&ta, a, M, K / 2, K / 2, 128, kBM)) return st;
   if (int st = make_tmap_2d_8bit(&tb, b, N, K / 2, K / 2, 128, BN / CG)) return st;
@@ -443,7 +457,8 @@ int launch_tiles(void* c, const void* a, const void* as, const void* b, const vo
     return st;
   if (int st = make_tmap_blocks512(&tsb, bs, (static_cast<uint64_t>(N) + 127) / 128 * sf_tiles_k, 2))
     return st;
-  if (int st = output_map<T>(&tc, c, M, N, &tma_store)) return st;
+  const uintptr_t start = reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(N * sizeof(T));
+  const int rows_on = start % 32 == 0 ? kRows32 : start % 16 == 0 ? kRows16 : kRowsAny;
   const int64_t tiles = tile_count(CG, BN, M, N);
   if (tiles > 0x3fffffffLL)
     return fail(AOTK_ERR_UNSUPPORTED, "aotk_mxfp4_gemm: output of %d x %d has too many tiles", M, N);
@@ -462,8 +477,8 @@ int launch_tiles(void* c, const void* a, const void* as, const void* b, const vo
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, tc, static_cast<T*>(c), M, N,
-                                     K, tma_store);
+  cudaError_t e =
+      cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, static_cast<T*>(c), M, N, K, rows_on);
   if (e != cudaSuccess)
     return fail(AOTK_ERR_CUDA, "aotk_mxfp4_gemm launch: %s", cudaGetErrorString(e));
   return check_launch("aotk_mxfp4_gemm");
@@ -481,11 +496,11 @@ int dispatch(void* c, const void* a, const void* as, const void* b, const void* 
   const double pairs = pair256 < pair128 ? pair256 : pair128;
   const double ones = one128 < one64 ? one128 : one64;
   if (pairs <= ones) {
-    if (pair256 <= pair128) return launch_tiles<T, 2, 256, 5>(c, a, as, b, bs, M, N, K, s, info);
-    return launch_tiles<T, 2, 128, 7>(c, a, as, b, bs, M, N, K, s, info);
+    if (pair256 <= pair128) return launch_tiles<T, 2, 256, 6>(c, a, as, b, bs, M, N, K, s, info);
+    return launch_tiles<T, 2, 128, 8>(c, a, as, b, bs, M, N, K, s, info);
   }
-  if (one128 <= one64) return launch_tiles<T, 1, 128, 5>(c, a, as, b, bs, M, N, K, s, info);
-  return launch_tiles<T, 1, 64, 7>(c, a, as, b, bs, M, N, K, s, info);
+  if (one128 <= one64) return launch_tiles<T, 1, 128, 6>(c, a, as, b, bs, M, N, K, s, info);
+  return launch_tiles<T, 1, 64, 8>(c, a, as, b, bs, M, N, K, s, info);
 }
 
 // Whether M <= 128 rows go to the kernel that splits K and streams the weight at two
