@@ -4,11 +4,12 @@
 //
 // Persistent tcgen05 kernel on tiles of 128 CG x BN of C, CG = 1 or 2 CTAs (SMs)
 // per tile:
-//   * codes are read as bytes by TMA, 256 elements of K (one 128-byte swizzle
-//     row) per stage, both operands K-major; scale tiles (512 bytes per 128 rows
-//     x 4 blocks, already in the order of TMEM) by TMA as rows of 512 bytes;
-//   * per stage one thread copies the scales to TMEM and issues up to four K = 64
-//     MMAs (kind::mxf4).  TMEM holds one scale area per stage of the ring, so a
+//   * codes are read as bytes by TMA in blocks of 256 elements of K (one 128-byte
+//     swizzle row), SUB blocks per stage, both operands K-major; scale tiles (512
+//     bytes per 128 rows x 4 blocks, already in the order of TMEM) by TMA as rows
+//     of 512 bytes;
+//   * per stage one thread copies the scales to TMEM and issues up to 4 SUB MMAs of
+//     K = 64 (kind::mxf4).  TMEM holds one scale area per stage of the ring, so a
 //     stage's scales are overwritten only when its barrier has shown that the
 //     MMAs which read them are done;
 //   * CG = 2 (cta_group::2): each CTA stages its 128 rows of A, BN / 2 of the rows
@@ -18,12 +19,15 @@
 //     BN = 256, so one accumulator is enough there (it and the scales would not
 //     fit twice into 512 columns); narrower tiles have two.  A lane holds a row and
 //     writes it in whole 32-byte sectors, without shared memory, which is the
-//     ring's (staged TMA stores and a stage less: 8192^3 226 -> 232 us, 128 x 6144 x
-//     4096 7.0 -> 7.1).  Where rows do not start on 16 bytes, the memory of two
-//     stages turns the rows for stores along them.
+//     ring's (staged TMA stores and a stage less: 8192^3 228 -> 232 us).  Where rows
+//     do not start on 16 bytes, the memory of one or two stages turns the rows for
+//     stores along them.
 // What bounds it: tiles of one CTA by operand traffic out of L2, about 16.5 TB/s
 // over the chip (128 x 256 tiles: 51 KB per 256 of K, 0.455 us where the MMAs take
-// 0.27); pairs of CTAs move 35 KB for the same work and end at the power cap.
+// 0.27); pairs of CTAs move 35 KB for the same work and end at the power cap.  64
+// columns are bound by the work per stage of the issuing warps, hence SUB = 2 there
+// (128 x 6144 x 4096 7.1 -> 6.6 us, 128 x 4096 x 14336 15.2 -> 13.3).  Sending the
+// scales a stage ahead of their MMAs, or between them, gained nothing or lost.
 // K is padded by zeros (TMA fill); MMAs stop at the last 64 elements that exist.
 // Rows beyond M or N may multiply stale or foreign scales, and are not stored.
 #include <type_traits>
@@ -51,28 +55,33 @@ constexpr uint32_t kScaleTile = 512;
 
 enum : unsigned { kWdProducer = 4096u, kWdMma = 8192u, kWdEpilogue = 16384u };
 
-template <int CG, int BN, int STAGES>
+// SUB: K blocks per stage.
+template <int CG, int BN, int STAGES, int SUB>
 struct MxLayout {
   static constexpr int kScaleTilesN = BN > 128 ? 2 : 1;  // scale tiles along N
-  static constexpr uint32_t kABytes = kBM * 128;
-  static constexpr uint32_t kBBytes = BN / CG * 128;
-  static constexpr uint32_t kSfBox = 2 * kScaleTile;  // both K tiles of a stage
+  static constexpr uint32_t kABlock = kBM * 128;
+  static constexpr uint32_t kBBlock = BN / CG * 128;
+  static constexpr uint32_t kABytes = SUB * kABlock;
+  static constexpr uint32_t kBBytes = SUB * kBBlock;
+  static constexpr uint32_t kSfBox = 2 * SUB * kScaleTile;  // the K tiles of a stage
   static constexpr uint32_t kSfBytes = (1 + kScaleTilesN) * kSfBox;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfBytes;
   static constexpr uint32_t kOffA = 0;
   static constexpr uint32_t kOffB = kOffA + STAGES * kABytes;
   static constexpr uint32_t kOffSf = kOffB + STAGES * kBBytes;
   static constexpr uint32_t kOffBar = kOffSf + STAGES * kSfBytes;
-  // Staging of unaligned rows: 4 KB per epilogue warp in A's last two stages.
+  // Staging of unaligned rows: 4 KB per epilogue warp in A's last one or two stages.
   static constexpr uint32_t kCBuf = 32 * 128;
-  static constexpr uint32_t kOffC = kOffA + (STAGES - 2) * kABytes;
-  static_assert(kEpiWarps * kCBuf <= 2 * kABytes, "staging fits two stages");
+  static constexpr int kStagingStages = kABytes >= kEpiWarps * kCBuf ? 1 : 2;
+  static constexpr uint32_t kOffC = kOffA + (STAGES - kStagingStages) * kABytes;
+  static_assert(kEpiWarps * kCBuf <= kStagingStages * kABytes, "staging fits");
+  static_assert(STAGES > kStagingStages + 1, "a ring is left beside the staging");
   static constexpr uint32_t kNumBars = 2 * STAGES + 5;  // full, empty, tfull x2, release x2, drain
   static constexpr uint32_t kOffMisc = kOffBar + kNumBars * 8;
   static constexpr uint32_t kAlloc = kOffMisc + 16 + 1024;
   static_assert(kAlloc <= 232448, "227 KB of shared memory");
   // TMEM columns: accumulators, then 4 columns per scale tile and stage.
-  static constexpr int kSfCols = 2 * 4 * (1 + kScaleTilesN);
+  static constexpr int kSfCols = 2 * SUB * 4 * (1 + kScaleTilesN);
   static constexpr int kAccs = 2 * BN + STAGES * kSfCols <= 512 ? 2 : 1;
   static constexpr int kSfBase = kAccs * BN;
   static constexpr int kTmemCols = kSfBase + STAGES * kSfCols > 256 ? 512 : 256;
@@ -155,14 +164,14 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ c, const uint32_t* r
   __syncwarp();
 }
 
-template <typename T, int CG, int BN, int STAGES>
+template <typename T, int CG, int BN, int STAGES, int SUB>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
                       const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmSa,
                       const __grid_constant__ CUtensorMap tmSb, T* __restrict__ c, int M, int N,
                       int K, int rows_on) {
-  using L = MxLayout<CG, BN, STAGES>;
+  using L = MxLayout<CG, BN, STAGES, SUB>;
   constexpr int kTileM = CG * kBM;
   constexpr int kGroup = kGroupRows / kTileM;
   constexpr int kChunk = 128 / sizeof(T);                // columns of 128 bytes of output
@@ -190,9 +199,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tiles_m = (M + kTileM - 1) / kTileM;
   const int tiles_n = (N + BN - 1) / BN;
   const int num_tiles = tiles_m * tiles_n;
-  const int kblocks = (K + kBK - 1) / kBK;
+  const int kblocks = (K + SUB * kBK - 1) / (SUB * kBK);  // stages
   const int sf_tiles_k = (K + 127) / 128;
-  const int stages = rows_on == kRowsAny ? STAGES - 2 : STAGES;
+  const int stages = rows_on == kRowsAny ? STAGES - L::kStagingStages : STAGES;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -250,8 +259,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int kb = 0; kb < kblocks; ++kb) {
         ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, wd, kWdProducer);
         if (!ok) break;
-        // Boxes of scales are always two tiles: the second may belong to the
-        // next 128 rows, or be zeros beyond the last.  No MMA reads it then.
+        // Boxes of scales are always 2 SUB tiles: the last may belong to the next
+        // 128 rows, or be zeros beyond the last.  No MMA reads them then.
         const uint32_t a_dst = base + L::kOffA + stage * L::kABytes;
         const uint32_t b_dst = base + L::kOffB + stage * L::kBBytes;
         const uint32_t sf = base + L::kOffSf + stage * L::kSfBytes;
@@ -259,21 +268,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), CG * L::kStageBytes);
           if constexpr (CG == 2) {
             const uint32_t fb = map_to_rank(full_bar(stage), 0);
-            tma_load_2d_pair(a_dst, &tmA, kb * 128, row_a, fb);
-            tma_load_2d_pair(b_dst, &tmB, kb * 128, row_b, fb);
-            tma_load_2d_pair(sf, &tmSa, 0, sa_row + 2 * kb, fb);
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) {
+              tma_load_2d_pair(a_dst + i * L::kABlock, &tmA, (kb * SUB + i) * 128, row_a, fb);
+              tma_load_2d_pair(b_dst + i * L::kBBlock, &tmB, (kb * SUB + i) * 128, row_b, fb);
+            }
+            tma_load_2d_pair(sf, &tmSa, 0, sa_row + 2 * SUB * kb, fb);
 #pragma unroll
             for (int j = 0; j < L::kScaleTilesN; ++j)
-              tma_load_2d_pair(sf + (1 + j) * L::kSfBox, &tmSb, 0, sb_row + j * sf_tiles_k + 2 * kb,
-                               fb);
+              tma_load_2d_pair(sf + (1 + j) * L::kSfBox, &tmSb, 0,
+                               sb_row + j * sf_tiles_k + 2 * SUB * kb, fb);
           } else {
             const uint32_t fb = full_bar(stage);
-            tma_load_2d(a_dst, &tmA, kb * 128, row_a, fb);
-            tma_load_2d(b_dst, &tmB, kb * 128, row_b, fb);
-            tma_load_2d(sf, &tmSa, 0, sa_row + 2 * kb, fb);
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) {
+              tma_load_2d(a_dst + i * L::kABlock, &tmA, (kb * SUB + i) * 128, row_a, fb);
+              tma_load_2d(b_dst + i * L::kBBlock, &tmB, (kb * SUB + i) * 128, row_b, fb);
+            }
+            tma_load_2d(sf, &tmSa, 0, sa_row + 2 * SUB * kb, fb);
 #pragma unroll
             for (int j = 0; j < L::kScaleTilesN; ++j)
-              tma_load_2d(sf + (1 + j) * L::kSfBox, &tmSb, 0, sb_row + j * sf_tiles_k + 2 * kb, fb);
+              tma_load_2d(sf + (1 + j) * L::kSfBox, &tmSb, 0,
+                          sb_row + j * sf_tiles_k + 2 * SUB * kb, fb);
           }
         }
         __syncwarp();
@@ -334,21 +350,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t sfa = tmem_base + L::kSfBase + stage * L::kSfCols;
-          const uint32_t sfb = sfa + 8;
+          const uint32_t sfb = sfa + 8 * SUB;
           const uint64_t sd = sdesc_scales(base + L::kOffSf + stage * L::kSfBytes);
           const uint64_t ad = sdesc_sw128(base + L::kOffA + stage * L::kABytes, 16, 1024);
           const uint64_t bd = sdesc_sw128(base + L::kOffB + stage * L::kBBytes, 16, 1024);
-          const int steps = min(kBK / kStepK, (K - kb * kBK + kStepK - 1) / kStepK);
+          const int steps =
+              min(SUB * kBK / kStepK, (K - kb * SUB * kBK + kStepK - 1) / kStepK);
           if (elected) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {  // halves of 128 elements: one scale tile each
+            for (int t = 0; t < 2 * SUB; ++t) {  // 128 elements: one scale tile each
               if (2 * t < steps) {
                 // Descriptors count addresses in units of 16 bytes.
                 copy_scales(sfa + 4 * t, sd + t * (kScaleTile / 16));
 #pragma unroll
                 for (int j = 0; j < L::kScaleTilesN; ++j)
                   copy_scales(sfb + 4 * (L::kScaleTilesN * t + j),
-                              sd + (2 * (j + 1) + t) * (kScaleTile / 16));
+                              sd + (2 * SUB * (j + 1) + t) * (kScaleTile / 16));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                   const int k = 2 * t + h;
@@ -356,10 +373,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t sfb_t = sfb + 4 * L::kScaleTilesN * t + sfb_shift;
                     const uint32_t idesc = idesc_mxf4(kTileM, BN, 2 * h);
                     const bool add = kb > 0 || k > 0;
+                    // Block k / 4 of the stage, 32 bytes on per step.
+                    const uint64_t ak = ad + (k / 4) * (L::kABlock / 16) + (k % 4) * 2;
+                    const uint64_t bk = bd + (k / 4) * (L::kBBlock / 16) + (k % 4) * 2;
                     if constexpr (CG == 2)
-                      umma_mxf4_pair(d_tmem, ad + k * 2, bd + k * 2, idesc, sfa + 4 * t, sfb_t, add);
+                      umma_mxf4_pair(d_tmem, ak, bk, idesc, sfa + 4 * t, sfb_t, add);
                     else
-                      umma_mxf4(d_tmem, ad + k * 2, bd + k * 2, idesc, sfa + 4 * t, sfb_t, add);
+                      umma_mxf4(d_tmem, ak, bk, idesc, sfa + 4 * t, sfb_t, add);
                   }
                 }
               }
@@ -443,19 +463,19 @@ int64_t tile_count(int cg, int bn, int M, int N) {
   return static_cast<int64_t>((M - 1) / (cg * kBM) + 1) * ((N - 1) / bn + 1);
 }
 
-template <typename T, int CG, int BN, int STAGES>
+template <typename T, int CG, int BN, int STAGES, int SUB>
 int launch_tiles(void* c, const void* a, const void* as, const void* b, const void* bs, int M,
                  int N, int K, cudaStream_t stream, const DeviceInfo& info) {
-  using L = MxLayout<CG, BN, STAGES>;
-  auto kernel = gemm_mxfp4_kernel<T, CG, BN, STAGES>;
+  using L = MxLayout<CG, BN, STAGES, SUB>;
+  auto kernel = gemm_mxfp4_kernel<T, CG, BN, STAGES, SUB>;
   if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kAlloc, info)) return st;
   CUtensorMap ta, tb, tsa, tsb;
   const uint64_t sf_tiles_k = (static_cast<uint64_t>(K) + 127) / 128;
   if (int st = make_tmap_2d_8bit(&ta, a, M, K / 2, K / 2, 128, kBM)) return st;
   if (int st = make_tmap_2d_8bit(&tb, b, N, K / 2, K / 2, 128, BN / CG)) return st;
-  if (int st = make_tmap_blocks512(&tsa, as, (static_cast<uint64_t>(M) + 127) / 128 * sf_tiles_k, 2))
+  if (int st = make_tmap_blocks512(&tsa, as, (static_cast<uint64_t>(M) + 127) / 128 * sf_tiles_k, 2 * SUB))
     return st;
-  if (int st = make_tmap_blocks512(&tsb, bs, (static_cast<uint64_t>(N) + 127) / 128 * sf_tiles_k, 2))
+  if (int st = make_tmap_blocks512(&tsb, bs, (static_cast<uint64_t>(N) + 127) / 128 * sf_tiles_k, 2 * SUB))
     return st;
   const uintptr_t start = reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(N * sizeof(T));
   const int rows_on = start % 32 == 0 ? kRows32 : start % 16 == 0 ? kRows16 : kRowsAny;
@@ -487,20 +507,22 @@ int launch_tiles(void* c, const void* a, const void* as, const void* b, const vo
 template <typename T>
 int dispatch(void* c, const void* a, const void* as, const void* b, const void* bs, int M, int N,
              int K, cudaStream_t s, const DeviceInfo& info) {
+  // Rounds of tiles on the SMs, times what a round takes against one of 256-column
+  // pairs (per 256 of K at full load 0.40 us; 0.29, 0.31 and 0.23 for the others).
   auto cost = [&](int cg, int bn, double round) {
     const int64_t workers = info.sm_count / cg;
     return round * static_cast<double>((tile_count(cg, bn, M, N) + workers - 1) / workers);
   };
   const double pair256 = cost(2, 256, 1.0), pair128 = cost(2, 128, 0.7);
-  const double one128 = cost(1, 128, 0.77), one64 = cost(1, 64, 0.65);
+  const double one128 = cost(1, 128, 0.77), one64 = cost(1, 64, 0.58);
   const double pairs = pair256 < pair128 ? pair256 : pair128;
   const double ones = one128 < one64 ? one128 : one64;
   if (pairs <= ones) {
-    if (pair256 <= pair128) return launch_tiles<T, 2, 256, 6>(c, a, as, b, bs, M, N, K, s, info);
-    return launch_tiles<T, 2, 128, 8>(c, a, as, b, bs, M, N, K, s, info);
+    if (pair256 <= pair128) return launch_tiles<T, 2, 256, 6, 1>(c, a, as, b, bs, M, N, K, s, info);
+    return launch_tiles<T, 2, 128, 8, 1>(c, a, as, b, bs, M, N, K, s, info);
   }
-  if (one128 <= one64) return launch_tiles<T, 1, 128, 6>(c, a, as, b, bs, M, N, K, s, info);
-  return launch_tiles<T, 1, 64, 8>(c, a, as, b, bs, M, N, K, s, info);
+  if (one128 <= one64) return launch_tiles<T, 1, 128, 6, 1>(c, a, as, b, bs, M, N, K, s, info);
+  return launch_tiles<T, 1, 64, 4, 2>(c, a, as, b, bs, M, N, K, s, info);
 }
 
 // Whether M <= 128 rows go to the kernel that splits K and streams the weight at two
@@ -508,9 +530,8 @@ int dispatch(void* c, const void* a, const void* as, const void* b, const void* 
 // partial sums grows with M, the latter go through K one block after the other; up
 // to 32 rows the former always won.  Estimates in us from graph replays on 148 SMs,
 // weight from HBM (split / 64-column tiles / 128-column tiles measured): 128 rows,
-// N x K = 6144 x 4096 12.3 / 7.1 / 7.8, 4096 x 14336 13.2 / 15.4 / 17.4, 8192 x 8192
-// 14.3 / 10.9 / 12.2, 1024 x 8192 8.2 / 10.0 / 11.1, 28672 x 4096 17.2 / 20.0 / 15.9;
-// 64 rows, 6144 x 4096 8.6 / 6.9 / 7.5, 28672 x 4096 14.5 / 19.0 / 15.0.
+// N x K = 6144 x 4096 12.3 / 6.6 / 7.6, 4096 x 14336 13.2 / 13.3 / 16.7, 28672 x 4096
+// 17.2 / 19.0 / 15.8, 1024 x 8192 8.2 / 9.0 / 11.1; 64 rows, 28672 x 4096 14.5 / 18 / 15.
 bool prefer_split(int M, int N, int K, const DeviceInfo& info) {
   if (M <= 32) return true;
   const double weight_kb = static_cast<double>(N) * K * (17.0 / 32) / 1024;
@@ -521,7 +542,7 @@ bool prefer_split(int M, int N, int K, const DeviceInfo& info) {
     const double stream = weight_kb / 5100;
     return 3.8 + (loop > stream ? loop : stream);
   };
-  const double t64 = tiles(64, 0.207), t128 = tiles(128, 0.241);
+  const double t64 = tiles(64, 0.167), t128 = tiles(128, 0.241);
   const double split = 2.5 + 0.039 * M + weight_kb / 4900;
   return split <= t64 && split <= t128;
 }
