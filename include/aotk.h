@@ -361,7 +361,8 @@ AOTK_API int aotk_gemm_schedule(int64_t M, int64_t N, int64_t K, int elem_bytes,
  * kernel: 1 producer, 2 MMA, 4 epilogue, 64 peer / flag wait, 128 self-test,
  * 2048 K-split partials; skinny kernel: 8, 16, 32; CTA-pair kernel: 256,
  * 512, 1024; 4-bit product: 4096, 8192, 16384, for
- * M <= 128 32768, 65536, 131072; sandwich norm: 262144.  Synchronises the device.  clear != 0 resets it to 0 after reading. */
+ * M <= 128 32768, 65536, 131072; sandwich norm: 262144.  Synchronises the
+ * device.  clear != 0 resets it to 0 after reading. */
 AOTK_API int aotk_watchdog_status(int device, uint32_t* status, int clear);
 
 /* Runs the kernels' bounded waits with nothing to wait for - an mbarrier
@@ -398,7 +399,9 @@ AOTK_API int aotk_mxfp4_dequantize(void* out, const void* codes, const void* sca
                                    int64_t cols, int dtype, void* stream);
 
 /* C[M, N] = A B^T over the values of A [M, K] and B [N, K] (both quantised
- * along K), fp32 accumulation, one rounding to out_dtype (fp32, fp16, bf16). */
+ * along K), fp32 accumulation, one rounding to out_dtype (fp32, fp16, bf16).
+ * K <= 2^28.  Where K is not a multiple of 64 the scales' padding is read, with
+ * elements that are 0: a padding byte of 255 would make the sums NaN. */
 AOTK_API int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, const void* b,
                              const void* b_scales, int64_t M, int64_t N, int64_t K, int out_dtype,
                              void* stream);

@@ -57,6 +57,8 @@ def mxfp4_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     float16 or float32).
 
     ``out`` may name a contiguous [M, N] tensor of dtype ``out_dtype`` to write into.
+    K is at most 2^28.  Scale bytes that pad the last tile of a row have to be 0, as
+    ``mxfp4_quantize`` and ``mxfp4_tile_scales`` write them.
     """
     if out is None:
         return _gemm(a, a_scales, b, b_scales, out_dtype)

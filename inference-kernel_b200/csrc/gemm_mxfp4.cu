@@ -52,6 +52,9 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer, MMA and epilogue warps
 constexpr int kGroupRows = 2048;  // rows of A per raster group
 constexpr uint32_t kScaleTile = 512;
+// A wait for a tile's whole sum lasts as long as K does.  The bound of all waits (2e9
+// cycles, sm100.cuh) must not end it: 2^20 K blocks take at most 0.9e9 cycles.
+constexpr int64_t kMaxK = int64_t{1} << 28;
 
 enum : unsigned { kWdProducer = 4096u, kWdMma = 8192u, kWdEpilogue = 16384u };
 
@@ -578,8 +581,10 @@ extern "C" int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, con
   if (M == 0 || N == 0) return AOTK_OK;
   if (!c || (K > 0 && (!a || !a_scales || !b || !b_scales)))
     return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  if (M > 0x7fffff00LL || N > 0x7fffff00LL || K > 0x7fffff00LL)
+  if (M > 0x7fffff00LL || N > 0x7fffff00LL)
     return fail(AOTK_ERR_UNSUPPORTED, "%s: extents above 2^31 - 256", who);
+  if (K > kMaxK)
+    return fail(AOTK_ERR_UNSUPPORTED, "%s: K = %lld is above 2^28", who, (long long)K);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (K == 0) {  // an empty sum
     const size_t bytes = static_cast<size_t>(M) * static_cast<size_t>(N) * elem_size(out_dtype);

@@ -68,7 +68,7 @@ struct MxsLayout {
 
 // Parts: unit x of U (K block x % kblocks of strip x / kblocks of the cluster's
 // strips) belongs to CTA part_of(x); CTA r has units [part_begin(r), part_begin(r + 1)).
-// U < 2^23 x 8 and C <= 8, so the products fit 32 bits.
+// K <= 2^28: U < 2^20 x 8 and C <= 8, so the products fit 32 bits.
 __device__ __forceinline__ int part_begin(int r, int units, int ctas) {
   return static_cast<int>(static_cast<unsigned>(units * r) / static_cast<unsigned>(ctas));
 }

@@ -117,3 +117,11 @@ def test_empty_problems_are_no_ops():
     capi.mxfp4_gemm(0, 0, 0, 0, 0, 0, 8, 64, BF16)
     capi.mxfp4_gemm(0, 0, 0, 0, 0, 8, 0, 64, BF16)
     capi.sandwich_rmsnorm(0, 0, 0, 0, 0, 0, None, 0, 0, 1.0, 0, 64, 1e-6, BF16)
+
+
+@pytest.mark.parametrize("K", [(1 << 28) + 32, 1 << 30, (1 << 31) - 256])
+def test_product_refuses_sums_longer_than_its_waits(K):
+    """Refused before any device is asked: a kernel's bounded waits would give up."""
+    with pytest.raises(capi.AotkError) as e:
+        capi.mxfp4_gemm(16, 16, 16, 16, 16, 4, 4, K, BF16)
+    assert e.value.status == capi.ERR_UNSUPPORTED and "2^28" in str(e.value)
