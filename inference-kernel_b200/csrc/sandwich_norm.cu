@@ -549,7 +549,13 @@ __global__ void __launch_bounds__(kRingThreads, 1)
       }
     }
     const float sum = group_sum<TPR>(ss.x + ss.y, partial[group][0], group, t, bad);
-    if (bad) break;  // the whole group
+    if (bad) {  // the whole group, once what it has requested has arrived
+      for (int k = 0; t == 0 && k < stages && row + k * step < a.rows; ++k) {
+        const bool wraps = stage + k >= stages;
+        mbar_drain(bar0 + 8u * (stage + k - (wraps ? stages : 0)), phase ^ (wraps ? 1u : 0u));
+      }
+      break;
+    }
     const float inv = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
 
     ss = make_float2(0.f, 0.f);
@@ -602,9 +608,6 @@ __global__ void __launch_bounds__(kRingThreads, 1)
       phase ^= 1u;
     }
   }
-  // After a wait that gave up, copies may still be in flight.
-  if (t == 0 && abort_flag)
-    for (int k = 0; k < stages; ++k) mbar_drain(bar0 + 8u * k, phase);
 }
 
 // Any row length and alignment: one block per row; h is computed again from its
