@@ -449,3 +449,107 @@ def test_block_in_four_bits(M):
     assert np.all(np.abs(np64(h) - hh) <= 2.0 ** -8 * np.abs(hh) + 1e-5)
     assert np.all(np.abs(np64(out) - o) <= 2.0 ** -8 * np.abs(o) + 1e-4)
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 40, 1 << 20), (130, 40, 1 << 20), (3, (1 << 20) + 5, 64),
+                                   (130, (1 << 19) + 8, 64), ((1 << 20) + 3, 24, 96)], ids=str)
+def test_gemm_long_sums_and_many_rows(M, N, K):
+    """Elements 0, +-.5 and +-1 at scale 1: any partial sum is a multiple of 1/4 and at
+    most K <= 2^20, so fp32 sums are exact in any order (22 bits)."""
+    import torch
+
+    import aot_kernel
+
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    element = torch.tensor([0.0, 0.5, 1.0, -0.5, -1.0], device="cuda")
+    code = torch.tensor([0, 1, 2, 9, 10], device="cuda", dtype=torch.uint8)
+
+    def operand(rows):
+        pick = torch.randint(0, 5, (rows, K), generator=gen, device="cuda")
+        codes = code[pick[:, ::2]] | code[pick[:, 1::2]] << 4
+        one = torch.full((rows, K // 32), 127, dtype=torch.uint8, device="cuda")
+        return (codes, aot_kernel.mxfp4_tile_scales(one)), element[pick]
+
+    a, av = operand(M)
+    b, bv = operand(N)
+    got = aot_kernel.mxfp4_gemm(*a, *b, torch.float32)
+    for r in range(0, M, 1 << 17):  # bounds the 64-bit temporaries
+        want = av[r:r + (1 << 17)].double() @ bv.double().t()
+        assert torch.equal(got[r:r + (1 << 17)].double(), want)
+
+
+@pytest.mark.parametrize("M", [5, 90, 300])
+def test_gemm_of_a_matrix_with_itself(M):
+    import torch
+
+    import aot_kernel
+
+    q, s = aot_kernel.mxfp4_quantize(to_device(randn((M, 320), M), "bfloat16"))
+    got = aot_kernel.mxfp4_gemm(q, s, q, s, torch.float32)
+    assert torch.equal(got, aot_kernel.mxfp4_gemm(q, s, q.clone(), s.clone(), torch.float32))
+    v = aot_kernel.mxfp4_dequantize(q, s, torch.float32).double()
+    # K = 320 additions, each off by at most one unit in the last place of sum |a| |b|
+    assert ((got.double() - v @ v.t()).abs() <= 320 * 2.0 ** -23 * (v.abs() @ v.abs().t())).all()
+
+
+def test_two_graphs_replayed_at_once():
+    """The products keep no workspace that two graphs could share."""
+    import torch
+
+    import aot_kernel
+
+    K, N = 2048, 1024
+    w = aot_kernel.mxfp4_quantize(to_device(randn((N, K), 1), "bfloat16"))
+    xs = [aot_kernel.mxfp4_quantize(to_device(randn((M, K), 2 + M), "bfloat16")) for M in (6, 6, 100, 200)]
+    want = [aot_kernel.mxfp4_gemm(*x, *w) for x in xs]
+    graphs, got = [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append([aot_kernel.mxfp4_gemm(*x, *w) for _ in range(3)])
+    streams = [torch.cuda.Stream() for _ in xs]
+    for g in got:
+        for t in g:
+            t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, v) for g, v in zip(got, want) for t in g)
+
+
+FIRST_CALL = """
+import torch, aot_kernel
+gen = torch.Generator(device="cuda").manual_seed(1)
+M, N, K = {M}, 264, 512
+x = torch.randn(M, K, generator=gen, device="cuda", dtype=torch.bfloat16)
+y = torch.randn(N, K, generator=gen, device="cuda", dtype=torch.bfloat16)
+r = torch.randn(M, N, generator=gen, device="cuda", dtype=torch.bfloat16)
+w = torch.ones(N, device="cuda", dtype=torch.bfloat16)
+def step():
+    a, b = aot_kernel.mxfp4_quantize(x), aot_kernel.mxfp4_quantize(y)
+    c = aot_kernel.mxfp4_gemm(*a, *b)
+    return c, aot_kernel.mxfp4_dequantize(*a), *aot_kernel.sandwich_rmsnorm(c, r, w, w)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+assert all(torch.equal(g, v) for g, v in zip(got, step()))
+print("replayed")
+"""
+
+
+@pytest.mark.parametrize("M", [4, 70, 2500])
+def test_first_call_may_be_captured(M):
+    """No call is needed before a capture (in a process of its own: nothing is loaded)."""
+    import os
+    import subprocess
+    import sys
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL.format(M=M)], capture_output=True,
+                          text=True, timeout=300,
+                          env=dict(os.environ, PYTHONPATH=os.pathsep.join(filter(None, sys.path))))
+    assert done.returncode == 0 and "replayed" in done.stdout, done.stderr[-2000:]

@@ -278,3 +278,52 @@ def test_offsets_beyond_32_bits(cols):
         for g, w in ((out, o), (h, hh)):  # sums in another order: at most one step of bf16
             g = g[r0:r0 + 9].double()
             assert ((g - w.double()).abs() <= 2.0 ** -7 * w.double().abs() + 1e-3).all()
+
+
+@pytest.mark.parametrize("shape", [(3, 100), (5, 512), (700, 1000), (700, 2048), (3, 40000)], ids=str)
+def test_one_tensor_in_every_place(shape):
+    """x is the residual and the gate too, and one weight serves both norms."""
+    d = make(shape, "bfloat16")
+    d["residual"] = d["gate"] = d["x"]
+    d["pre"] = d["post"]
+    import torch
+
+    import aot_kernel
+
+    x, w = to_device(d["x"], "bfloat16"), to_device(d["post"], "bfloat16")
+    out, h = aot_kernel.sandwich_rmsnorm(x, x, w, w, EPS, gate=x)
+    o2, h2 = check(d, "bfloat16")
+    assert torch.equal(out, o2) and torch.equal(h, h2)
+
+
+@pytest.mark.parametrize("cols", [1000, 1003])
+def test_graph_of_many_rows(cols):
+    """Captured and replayed with new inputs; two replays in flight on two streams."""
+    import torch
+
+    import aot_kernel
+
+    sets = [{k: to_device(v, "bfloat16") for k, v in make((900, cols), "bfloat16", (900, 1), s).items()}
+            for s in (10, 20)]
+
+    def step(d):
+        return aot_kernel.sandwich_rmsnorm(d["x"], d["residual"], d["post"], d["pre"], EPS,
+                                           gate=d["gate"])
+
+    graphs, got = [], []
+    for d in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(step(d))
+    for d in sets:
+        d["x"].neg_()
+    want = [step(d) for d in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
