@@ -12,7 +12,11 @@
 //     CTAs that hold parts of the same strip (st.async), each of which receives the
 //     strip's columns of its own, adds them in rank order, rounds and writes them:
 //     no workspace, no atomics, one launch, the same sum every time.  Nobody waits
-//     for a cluster barrier at the end; a CTA leaves when it has what is sent to it.
+//     for a cluster barrier at the end; a CTA leaves when it has what is sent to it;
+//   * a CTA asks for its first blocks of the weight in L2 before it waits for the
+//     previous kernel on the stream (kAhead; graph replays, us: 1 x 28672 x 4096
+//     12.6 -> 12.0, 1 x 6144 x 4096 5.45 -> 4.9, 1 x 4096 x 14336 8.0 -> 7.3, after a
+//     quantiser 10.2 -> 9.3).
 // Stages, scale copies and scale areas in TMEM are those of gemm_mxfp4.cu.
 #include "common.h"
 #include "gemm_internal.h"
@@ -32,6 +36,7 @@ constexpr int kTileN = 128;    // rows of B per strip (the MMA's M)
 constexpr int kBK = 256;       // elements of K per stage (128 bytes of codes)
 constexpr int kStepK = 64;
 constexpr int kMaxCluster = 8;
+constexpr int kAhead = 4;      // blocks prefetched; 2 gain less, 8 or all of them lose at 48 rows
 constexpr uint32_t kScaleTile = 512;
 
 enum : unsigned { kWdProducer = 32768u, kWdMma = 65536u, kWdEpilogue = 131072u };
@@ -153,6 +158,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 1) {
     tmem_alloc(smem_addr(tmem_slot), L::kTmemCols);
     tmem_relinquish();
+  } else if (warp == 2) {
+    if (elect_one()) {
+      int strip = strip0 + local0, kb = u0 - local0 * kblocks;
+      for (int u = u0; u < min(u1, u0 + kAhead); ++u) {
+        tma_prefetch_2d(&tmW, kb * 128, strip * kTileN);
+        const int sk = 2 * kb;
+        bulk_prefetch(w_scales + (static_cast<int64_t>(strip) * sf_tiles_k + sk) * kScaleTile,
+                      (sk + 1 < sf_tiles_k ? 2 : 1) * kScaleTile);
+        if (++kb == kblocks) {
+          kb = 0;
+          ++strip;
+        }
+      }
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
