@@ -170,64 +170,52 @@ struct Block {
   }
 };
 
-// Items (blocks) per thread when quantising: 128 bytes in flight.
-template <typename T>
-constexpr int kItems = 4 / sizeof(T);
-
+// One block per thread: the next ones come with the SM's other thread blocks, and a
+// problem of few waves ends evenly (two per thread, 16-bit types: 1024 x 4096 3.7 ->
+// 4.8 us, 4096 x 8192 14.1 -> 14.7, 1 x 4096 1.4 -> 1.7).
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                     const T* __restrict__ x, int64_t stride, int64_t rows, int64_t rows_padded,
                     int cols, const Walk walk) {
-  constexpr int U = kItems<T>;
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
-  Block<T> in[U];
-  int64_t row[U];
-  int kb[U];
-  first_item<U>(walk, row[0], kb[0]);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (u > 0) {
-      row[u] = row[u - 1];
-      kb[u] = kb[u - 1];
-      next_item(walk, row[u], kb[u]);
-    }
-    if (row[u] < rows && kb[u] * 32 < cols) {
-      const T* p = x + row[u] * stride + kb[u] * 32;
-      if constexpr (kAligned)
-        in[u].load(p);
-      else
-        in[u].load_any(p, x, x + (rows - 1) * stride + cols);
-    } else {
-      in[u].zero();
-    }
+  int64_t row;
+  int kb;
+  first_item<1>(walk, row, kb);
+  const bool live = row < rows && kb * 32 < cols;
+  Block<T> in;
+  if (live) {
+    const T* p = x + row * stride + kb * 32;
+    if constexpr (kAligned)
+      in.load(p);
+    else
+      in.load_any(p, x, x + (rows - 1) * stride + cols);
+  } else {
+    in.zero();
   }
+  const uint32_t e = in.top_exponent();
+  const bool bad = e == 255;
+  const uint32_t byte = bad ? 255u : e > 2 ? e - 2 : 0u;
+  const float inv = __uint_as_float((254u - (bad ? 0u : byte)) << 23);
+  uint32_t word[4];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t e = in[u].top_exponent();
-    const bool bad = e == 255;
-    const uint32_t byte = bad ? 255u : e > 2 ? e - 2 : 0u;
-    const float inv = __uint_as_float((254u - (bad ? 0u : byte)) << 23);
-    uint32_t word[4];
+  for (int i = 0; i < 4; ++i) {
+    float f[8];
+    in.get8(i, f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[8];
-      in[u].get8(i, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= inv;
-      word[i] = bad ? 0u : mx::encode_e2m1x8(f);
-    }
-    // Four neighbours are a row's four blocks of one scale tile.
-    uint32_t four = byte << ((threadIdx.x & 3) * 8);
-    four |= __shfl_xor_sync(0xffffffffu, four, 1);
-    four |= __shfl_xor_sync(0xffffffffu, four, 2);
-    if (row[u] < rows && kb[u] * 32 < cols)
-      *reinterpret_cast<uint4*>(codes + row[u] * (cols / 2) + kb[u] * 16) =
-          make_uint4(word[0], word[1], word[2], word[3]);
-    if ((threadIdx.x & 3) == 0 && row[u] < rows_padded)
-      *reinterpret_cast<uint32_t*>(scales + scale_byte(row[u], kb[u], walk.items_k)) = four;
+    for (int j = 0; j < 8; ++j) f[j] *= inv;
+    word[i] = bad ? 0u : mx::encode_e2m1x8(f);
   }
+  // Four neighbours are a row's four blocks of one scale tile.
+  uint32_t four = byte << ((threadIdx.x & 3) * 8);
+  four |= __shfl_xor_sync(0xffffffffu, four, 1);
+  four |= __shfl_xor_sync(0xffffffffu, four, 2);
+  if (live)
+    *reinterpret_cast<uint4*>(codes + row * (cols / 2) + kb * 16) =
+        make_uint4(word[0], word[1], word[2], word[3]);
+  if ((threadIdx.x & 3) == 0 && row < rows_padded)
+    *reinterpret_cast<uint32_t*>(scales + scale_byte(row, kb, walk.items_k)) = four;
 }
 
 // Elements per item when reading back: 32 bytes of output, so that a warp's
@@ -235,7 +223,9 @@ __global__ void __launch_bounds__(kThreads)
 // fp32, and too few threads where there is little to do).
 template <typename T>
 constexpr int kOutItem = 32 / sizeof(T);
-constexpr int kOutUnroll = 4;
+// Items per thread (1024 x 4096 bf16 with 1 / 2 / 4: 3.3 / 3.8 / 4.8 us, 4096 x 8192
+// 14.2 / 12.3 / 12.1, 14336 x 4096 fp32 46.2 / 42.1 / 42.9).
+constexpr int kOutUnroll = 2;
 
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
@@ -335,7 +325,7 @@ int quantize(void* codes, void* scales, const void* x, int64_t stride, int64_t r
   const Walk walk = walk_of(cols, 32);
   const int64_t padded = (rows + 127) / 128 * 128;
   auto run = [&](auto kernel) {
-    return launch("aotk_mxfp4_quantize", kernel, padded * walk.items_k, kItems<T>, s,
+    return launch("aotk_mxfp4_quantize", kernel, padded * walk.items_k, 1, s,
                   static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
                   static_cast<const T*>(x), stride, rows, padded, static_cast<int>(cols), walk);
   };
