@@ -111,11 +111,44 @@ __device__ __forceinline__ uint32_t pack_word(const uint32_t* r, int i) {
     return Elem<T>::pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 
-enum : int { kRowsAny = 0, kRows16 = 1, kRows32 = 2 };  // bytes that rows of C start on
+enum : int { kRowsAny = 0, kRows4 = 1, kRows16 = 2, kRows32 = 3 };  // bytes that rows of C start on
+
+// Writes `bytes` of each staged row of 128 bytes as units of type U along the rows,
+// whole rows several at a time.
+template <typename U>
+__device__ __forceinline__ void write_rows(uint8_t* p, int64_t pitch, const uint8_t* buf, int lane,
+                                           int bytes, int rows) {
+  constexpr int kUnits = 4 / sizeof(U);  // per lane and row
+  constexpr int kRows = 8 / kUnits;
+  auto at = [&](int k) { return (lane + 32 * k) * static_cast<int>(sizeof(U)); };
+  auto unit = [&](int rr, int k) {
+    return *reinterpret_cast<const U*>(buf + rr * 128 + ((at(k) / 16 ^ (rr & 7)) << 4) + at(k) % 16);
+  };
+  int rr = 0;
+  if (bytes == 128) {
+    for (; rr + kRows <= rows; rr += kRows, p += kRows * pitch) {
+      U v[kRows][kUnits];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) v[i][k] = unit(rr + i, k);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) *reinterpret_cast<U*>(p + i * pitch + at(k)) = v[i][k];
+    }
+  }
+  for (; rr < rows; ++rr, p += pitch)
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k)
+      if (at(k) < bytes) *reinterpret_cast<U*>(p + at(k)) = unit(rr, k);
+}
 
 // Writes a warp's 32 rows x 128 bytes of accumulators (lane = row) to C at (x, y).
 // A lane writes its row's vectors; rows that do not start on 16 bytes are turned
-// through 4 KB of shared memory and written element by element along the row.
+// through 4 KB of shared memory and written along the row in words, if they start on
+// 4 bytes, or elements (900 x 28611 x 832 to fp32 from row by row 57 -> 43 us, whole
+// sectors 33; bf16 31, 24; pure writes run at about 3.7 TB/s).
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* __restrict__ c, const uint32_t* r, uint8_t* buf,
                                             int lane, int x, int y, int M, int N, int rows_on) {
@@ -125,7 +158,7 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ c, const uint32_t* r
     return make_uint4(pack_word<T>(r, 4 * j), pack_word<T>(r, 4 * j + 1), pack_word<T>(r, 4 * j + 2),
                       pack_word<T>(r, 4 * j + 3));
   };
-  if (rows_on != kRowsAny) {
+  if (rows_on >= kRows16) {
     if (y + lane >= M) return;
     T* p = c + static_cast<int64_t>(y + lane) * N + x;
     auto one = [&](int j) {
@@ -153,17 +186,13 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ c, const uint32_t* r
   for (int j = 0; j < 8; ++j)
     *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = vec(j);
   __syncwarp();
-  const int rows = min(32, M - y);
-  for (int rr = 0; rr < rows; ++rr) {
-    T* crow = c + static_cast<int64_t>(y + rr) * N + x;
-#pragma unroll
-    for (int e = lane; e < kChunk; e += 32) {
-      const int b = e * static_cast<int>(sizeof(T));
-      const T v =
-          *reinterpret_cast<const T*>(buf + rr * 128 + (((b >> 4) ^ (rr & 7)) << 4) + (b & 15));
-      if (x + e < N) crow[e] = v;
-    }
-  }
+  const int rows = min(32, M - y), bytes = min(kChunk, N - x) * static_cast<int>(sizeof(T));
+  uint8_t* p = reinterpret_cast<uint8_t*>(c + static_cast<int64_t>(y) * N + x);
+  const int64_t pitch = static_cast<int64_t>(N) * sizeof(T);
+  if (sizeof(T) == 4 || rows_on == kRows4)
+    write_rows<uint32_t>(p, pitch, buf, lane, bytes, rows);
+  else
+    write_rows<uint16_t>(p, pitch, buf, lane, bytes, rows);
   __syncwarp();
 }
 
@@ -204,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int num_tiles = tiles_m * tiles_n;
   const int kblocks = (K + SUB * kBK - 1) / (SUB * kBK);  // stages
   const int sf_tiles_k = (K + 127) / 128;
-  const int stages = rows_on == kRowsAny ? STAGES - L::kStagingStages : STAGES;
+  const int stages = rows_on < kRows16 ? STAGES - L::kStagingStages : STAGES;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -481,7 +510,8 @@ int launch_tiles(void* c, const void* a, const void* as, const void* b, const vo
   if (int st = make_tmap_blocks512(&tsb, bs, (static_cast<uint64_t>(N) + 127) / 128 * sf_tiles_k, 2 * SUB))
     return st;
   const uintptr_t start = reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(N * sizeof(T));
-  const int rows_on = start % 32 == 0 ? kRows32 : start % 16 == 0 ? kRows16 : kRowsAny;
+  const int rows_on = start % 32 == 0 ? kRows32 : start % 16 == 0 ? kRows16
+                      : start % 4 == 0 ? kRows4 : kRowsAny;
   const int64_t tiles = tile_count(CG, BN, M, N);
   if (tiles > 0x3fffffffLL)
     return fail(AOTK_ERR_UNSUPPORTED, "aotk_mxfp4_gemm: output of %d x %d has too many tiles", M, N);

@@ -553,3 +553,20 @@ def test_first_call_may_be_captured(M):
                           text=True, timeout=300,
                           env=dict(os.environ, PYTHONPATH=os.pathsep.join(filter(None, sys.path))))
     assert done.returncode == 0 and "replayed" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("N", [1, 2, 3, 31, 66, 127, 130, 190, 1002, 1004])
+@pytest.mark.parametrize("start", [0, 1, 2, 4, 8])
+def test_gemm_rows_that_start_anywhere(N, start, dtype):
+    """`out` from element `start` of a buffer on, rows of N elements, ragged last rows;
+    what lies before and behind stays as it was."""
+    import torch
+
+    for M, K in ((139, 96), (300, 64), (9, 64)):
+        a, b = held(M, K, 21, 1), held(N, K, 22, 1)
+        buf = torch.full((start + M * N + 64,), 7.0, dtype=torch_dtype(dtype), device="cuda")
+        product(a, b, dtype, out=buf[start:start + M * N].view(M, N))
+        want = torch.from_numpy(ops.mxfp4_values(*a) @ ops.mxfp4_values(*b).T).float()
+        got = buf.cpu()
+        assert torch.equal(got[start:start + M * N].view(M, N), want.to(torch_dtype(dtype)))
+        assert (got[:start] == 7).all() and (got[start + M * N:] == 7).all()
