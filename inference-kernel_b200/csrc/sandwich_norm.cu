@@ -211,9 +211,12 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
   auto first = [&](int c) { return kShift && c < 0 ? -c : 0; };
   auto last = [&](int c) { return kShift && a.cols - c < E ? a.cols - c : E; };
   auto row_vec = [&](const T* p, int c) {
-    if constexpr (kShift)
-      if (off + c + E > total) return gather(p, off + c, first(c), last(c));
-    return ld_stream(reinterpret_cast<const uint4*>(p + off + c));
+    int64_t at = off + c;
+    if constexpr (kShift) {
+      if (total < E) return make_uint4(0u, 0u, 0u, 0u);
+      at = min(at, (total & ~static_cast<int64_t>(E - 1)) - E);
+    }
+    return ld_stream(reinterpret_cast<const uint4*>(p + at));
   };
   auto gate_vec = [&](int c) {
     if constexpr (kShift) return load_shifted(gate, gate_at + c, a.gate.total, first(c), last(c));
@@ -252,6 +255,23 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
       res[i] = row_vec(a.residual, column(i));
     }
   }
+  // The tensor's last elements, if they lie behind its last whole vector (not where the
+  // row is loaded: behind a branch each vector there waits for its own load, 61 x 2047
+  // bf16 4.4 -> 5.3 us).
+  auto load_rest = [&]() {
+    if constexpr (kShift) {
+      if (off + a.cols > (total & ~static_cast<int64_t>(E - 1))) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int c = column(i);
+          if (used(i) && off + c + E > total) {
+            x[i] = gather(a.x, off + c, first(c), last(c));
+            res[i] = gather(a.residual, off + c, first(c), last(c));
+          }
+        }
+      }
+    }
+  };
   const ShiftedWeight<T> post_w(a.post, a.cols, skip), pre_w(a.pre, a.cols, skip);
   auto weight_vec = [&](const ShiftedWeight<T>& w, int i) {
     if constexpr (kShift) return w.at(t + i * TPR);
@@ -272,6 +292,7 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
     }
   }
 
+  load_rest();
   float2 h[VPT][P];  // x, then h
   float2 ss = make_float2(0.f, 0.f);
 #pragma unroll

@@ -327,3 +327,9 @@ def test_graph_of_many_rows(cols):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("cols", [1, 2, 3, 5, 7, 9, 11, 13, 15, 17, 2045])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 6, 7, 8, 33])
+def test_tensor_ends_anywhere_in_a_vector(rows, cols, dtype):
+    check(make((rows, cols), dtype, (1, cols), rows + cols), dtype)
