@@ -11,7 +11,8 @@
 //   * sandwich_kernel: TPR threads per row hold it in registers, everything
 //     requested before the first sum: few rows, and rows of any length whose
 //     starts are not multiples of 16 bytes;
-//   * sandwich_ring_kernel: many rows of 1 to 32 KB, streamed through shared memory;
+//   * sandwich_ring_kernel: many rows of 1 to 48 KB (32 KB where they do not start on
+//     16 bytes), streamed through shared memory;
 //   * sandwich_long_kernel: rows that fit neither, or tensors that do not start
 //     on 16 bytes: the row is read three times.
 //
@@ -360,7 +361,9 @@ constexpr int kRingThreads = 512;
 constexpr int kRingBytes = 196608;
 constexpr int kMaxStages = 8;
 constexpr int64_t kRingMinRow = 1024, kRingMinTotal = 1 << 20;  // bytes
-constexpr int64_t kRingMaxVectors = 4 * kRingThreads;           // of a row
+// Vectors of a row: as many as two stages hold, or as a thread holds with its weights.
+template <bool kShift>
+constexpr int64_t kRingMaxVectors = (kShift ? 4 : 6) * kRingThreads;
 
 __device__ unsigned g_norm_watchdog;
 enum : unsigned { kWdRow = 262144u };
@@ -495,11 +498,21 @@ __global__ void __launch_bounds__(kRingThreads, 1)
 
   // A thread's columns are the same in every row, so their weights stay in
   // registers (from L2 they would be as many bytes per row as x and the residual),
-  // and so does the gate until its row changes.
-  uint4 post[VPT], pre[VPT], g[VPT];
+  // and so does the gate until its row changes.  Weights of more than four vectors do
+  // not fit there and are read again for every row, which is still better than a row
+  // at a time in the registers of 1024 threads (1024 x 20480 bf16 56 -> 32 us).
+  constexpr bool kKeep = VPT <= 4;
+  static_assert(kKeep || !kShift, "shifted once");
+  uint4 post[kKeep ? VPT : 1], pre[kKeep ? VPT : 1], g[VPT];
+  auto weight = [&](const uint4* kept, const T* w, int i) {
+    if constexpr (kKeep)
+      return kept[i];
+    else
+      return ld_cached(reinterpret_cast<const uint4*>(w) + t + i * TPR);
+  };
   float g_row = 1.f;
   int64_t g_at = 0, g_end = 0;  // the gate row in use, the first row beyond it
-  {
+  if constexpr (kKeep) {
     const ShiftedWeight<T> post_w(a.post, a.cols, skip), pre_w(a.pre, a.cols, skip);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -597,7 +610,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(post[i], &w[0].x);
+        Elem<T>::unpack(weight(post, a.post, i), &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) h[i][e] = mul2(mul2(h[i][e], scale2), w[e]);
         if (gate_cols) {
@@ -623,7 +636,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(pre[i], &w[0].x);
+        Elem<T>::unpack(weight(pre, a.pre, i), &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) w[e] = mul2(mul2(h[i][e], inv_h2), w[e]);
         write(a.out, 1, i, w);
@@ -805,6 +818,8 @@ int dispatch_group(const Args<T>& a, int n, cudaStream_t s, const DeviceInfo& in
   if (n <= 3 * TPR) return launch_ring<T, kShift, 3, TPR>(a, s, info);
   if constexpr (sizeof(T) == 4 || TPR == kRingThreads)
     if (n <= 4 * TPR) return launch_ring<T, kShift, 4, TPR>(a, s, info);
+  if constexpr (TPR == kRingThreads && !kShift)
+    if (n <= 6 * TPR) return launch_ring<T, kShift, 6, TPR>(a, s, info);
   if constexpr (TPR < kRingThreads) return dispatch_group<T, kShift, TPR * 2>(a, n, s, info);
   return fail(AOTK_ERR_UNSUPPORTED, "aotk_sandwich_rmsnorm: row of %d vectors", n);
 }
@@ -835,7 +850,8 @@ int launch(void* out, void* h_out, const void* x, const void* residual, const vo
   const bool shift = cols % E != 0;
   const int64_t row_bytes = cols * static_cast<int64_t>(sizeof(T));
   const int64_t vectors = (cols + (shift ? 2 * (E - 1) : 0)) / E;
-  if (row_bytes >= kRingMinRow && vectors <= kRingMaxVectors && rows * row_bytes >= kRingMinTotal)
+  const int64_t most = shift ? kRingMaxVectors<true> : kRingMaxVectors<false>;
+  if (row_bytes >= kRingMinRow && vectors <= most && rows * row_bytes >= kRingMinTotal)
     return shift ? dispatch_ring<T, true>(a, s, info) : dispatch_ring<T, false>(a, s, info);
   return shift ? dispatch_rows<T, true>(a, s) : dispatch_rows<T, false>(a, s);
 }

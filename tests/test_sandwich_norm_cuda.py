@@ -333,3 +333,10 @@ def test_graph_of_many_rows(cols):
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 6, 7, 8, 33])
 def test_tensor_ends_anywhere_in_a_vector(rows, cols, dtype):
     check(make((rows, cols), dtype, (1, cols), rows + cols), dtype)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "group"])
+@pytest.mark.parametrize("cols", [9000, 10240, 16392, 20480, 24568, 24584])
+def test_many_long_rows(cols, gate, dtype):
+    shape = {"none": None, "channel": (1, cols), "group": (12, 1, cols)}[gate]
+    check(make((12, 27, cols), dtype, shape, cols), dtype, alpha=0.7)
