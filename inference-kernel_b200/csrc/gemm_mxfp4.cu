@@ -114,7 +114,7 @@ __device__ __forceinline__ uint32_t pack_word(const uint32_t* r, int i) {
 enum : int { kRowsAny = 0, kRows4 = 1, kRows16 = 2, kRows32 = 3 };  // bytes that rows of C start on
 
 // Writes `bytes` of each staged row of 128 bytes as units of type U along the rows,
-// whole rows several at a time.
+// eight units per lane at a time.
 template <typename U>
 __device__ __forceinline__ void write_rows(uint8_t* p, int64_t pitch, const uint8_t* buf, int lane,
                                            int bytes, int rows) {
@@ -125,17 +125,23 @@ __device__ __forceinline__ void write_rows(uint8_t* p, int64_t pitch, const uint
     return *reinterpret_cast<const U*>(buf + rr * 128 + ((at(k) / 16 ^ (rr & 7)) << 4) + at(k) % 16);
   };
   int rr = 0;
-  if (bytes == 128) {
-    for (; rr + kRows <= rows; rr += kRows, p += kRows * pitch) {
-      U v[kRows][kUnits];
+  for (; rr + kRows <= rows; rr += kRows, p += kRows * pitch) {
+    U v[kRows][kUnits];
 #pragma unroll
-      for (int i = 0; i < kRows; ++i)
+    for (int i = 0; i < kRows; ++i)
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) v[i][k] = unit(rr + i, k);
+      for (int k = 0; k < kUnits; ++k) v[i][k] = unit(rr + i, k);
+    if (bytes == 128) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i)
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) *reinterpret_cast<U*>(p + i * pitch + at(k)) = v[i][k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k)
+        if (at(k) < bytes)
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) *reinterpret_cast<U*>(p + i * pitch + at(k)) = v[i][k];
     }
   }
   for (; rr < rows; ++rr, p += pitch)
