@@ -570,3 +570,31 @@ def test_gemm_rows_that_start_anywhere(N, start, dtype):
         got = buf.cpu()
         assert torch.equal(got[start:start + M * N].view(M, N), want.to(torch_dtype(dtype)))
         assert (got[:start] == 7).all() and (got[start + M * N:] == 7).all()
+
+
+@pytest.mark.parametrize("M", [1, 30, 60, 128, 400])
+def test_operands_written_by_the_kernel_before(M):
+    """The weight is quantised by the launch right before the product that reads it."""
+    import torch
+
+    import aot_kernel
+
+    K, N = 1024, 4096
+    x = aot_kernel.mxfp4_quantize(to_device(randn((M, K), 1), "bfloat16"))
+    ws = [to_device(randn((N, K), 2 + i), "bfloat16") for i in range(3)]
+    want = []
+    for w in ws:
+        q = aot_kernel.mxfp4_quantize(w)
+        torch.cuda.synchronize()
+        want.append(aot_kernel.mxfp4_gemm(*x, *q))
+        torch.cuda.synchronize()
+    w = torch.empty_like(ws[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = aot_kernel.mxfp4_gemm(*x, *aot_kernel.mxfp4_quantize(w))
+    for _ in range(10):
+        for i, v in enumerate(ws):
+            w.copy_(v)
+            assert torch.equal(aot_kernel.mxfp4_gemm(*x, *aot_kernel.mxfp4_quantize(w)), want[i])
+            graph.replay()
+            assert torch.equal(got, want[i])

@@ -340,3 +340,35 @@ def test_tensor_ends_anywhere_in_a_vector(rows, cols, dtype):
 def test_many_long_rows(cols, gate, dtype):
     shape = {"none": None, "channel": (1, cols), "group": (12, 1, cols)}[gate]
     check(make((12, 27, cols), dtype, shape, cols), dtype, alpha=0.7)
+
+
+@pytest.mark.parametrize("cols", [4096, 1001, 20480, 640])
+def test_residual_written_by_the_kernel_before(cols):
+    """A chain of norms, each reading what the one before has just written (eagerly and
+    captured, with nothing between the launches), against the same chain with waits."""
+    import torch
+
+    import aot_kernel
+
+    d = {k: to_device(v, "bfloat16") for k, v in make((600, cols), "bfloat16").items()}
+
+    def chain(wait):
+        x, h, kept = d["x"], d["residual"], []
+        for _ in range(6):
+            x, h = aot_kernel.sandwich_rmsnorm(x, h, d["post"], d["pre"], EPS, residual_scale=0.9)
+            kept += [x, h]
+            if wait:
+                torch.cuda.synchronize()
+        return kept
+
+    want = chain(True)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(False)
+    for _ in range(5):
+        for t in got:
+            t.fill_(7)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
