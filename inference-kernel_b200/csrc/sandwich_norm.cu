@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
   }
   // The tensor's last elements, if they lie behind its last whole vector (not where the
   // row is loaded: behind a branch each vector there waits for its own load, 61 x 2047
-  // bf16 4.4 -> 5.3 us).
+  // bf16 4.4 -> 5.3 us with four vectors per thread).
   auto load_rest = [&]() {
     if constexpr (kShift) {
       if (off + a.cols > (total & ~static_cast<int64_t>(E - 1))) {
@@ -759,20 +759,29 @@ int launch_long(const Args<T>& a, cudaStream_t s) {
   return launch_kernel<T>(sandwich_long_kernel<T, E>, a, a.rows, kLongThreads, s);
 }
 
-// The smallest group of threads that holds a row in at most four vectors each.
+// The smallest group of threads that holds a row in at most two vectors each: with
+// four there was more to do behind every wait (16 x 4096 bf16 2.7 -> 2.1 us, 100 x 2048
+// 2.8 -> 2.1, 61 x 2047 4.6 -> 3.4, 16384 x 256 7.9 -> 6.9).  Rows of 8 to 16 vectors
+// stay with 8 threads, which many rows want (32768 x 128 6.6 us, 16 threads 7.5).  Of
+// the longest, 16-bit rows take 1024 threads (1 x 16384 8.6 -> 4.1) and fp32 rows
+// 512 with four vectors (1 x 8192 3.2, 3.8 with 1024).
 template <typename T, bool kShift>
 int dispatch_rows(const Args<T>& a, cudaStream_t s) {
   constexpr int E = Elem<T>::kPerVec;
   const int64_t n = (static_cast<int64_t>(a.cols) + (kShift ? 2 * (E - 1) : 0)) / E;  // at most
   if (n <= 8) return launch_rows<T, kShift, 1, 8>(a, s);
   if (n <= 16) return launch_rows<T, kShift, 2, 8>(a, s);
-  if (n <= 32) return launch_rows<T, kShift, 4, 8>(a, s);
+  if (n <= 32) return launch_rows<T, kShift, 2, 16>(a, s);
   if (n <= 64) return launch_rows<T, kShift, 2, 32>(a, s);
-  if (n <= 128) return launch_rows<T, kShift, 4, 32>(a, s);
-  if (n <= 256) return launch_rows<T, kShift, 4, 64>(a, s);
-  if (n <= 512) return launch_rows<T, kShift, 4, 128>(a, s);
-  if (n <= 1024) return launch_rows<T, kShift, 4, 256>(a, s);
-  if (n <= 2048) return launch_rows<T, kShift, 4, 512>(a, s);
+  if (n <= 128) return launch_rows<T, kShift, 2, 64>(a, s);
+  if (n <= 256) return launch_rows<T, kShift, 2, 128>(a, s);
+  if (n <= 512) return launch_rows<T, kShift, 2, 256>(a, s);
+  if (n <= 1024) return launch_rows<T, kShift, 2, 512>(a, s);
+  if constexpr (sizeof(T) == 2) {
+    if (n <= 2048) return launch_rows<T, kShift, 2, 1024>(a, s);
+  } else {
+    if (n <= 2048) return launch_rows<T, kShift, 4, 512>(a, s);
+  }
   if (n <= 4096) return launch_rows<T, kShift, 4, 1024>(a, s);
   return kShift ? launch_long<T, 1>(a, s) : launch_long<T, E>(a, s);
 }
