@@ -382,7 +382,7 @@ AOTK_API int aotk_watchdog_selftest(void* stream);
  *          (r % 32) * 16 + (r % 128 / 32) * 4 + j % 4 of tile
  *          [r / 128][j / 4]; it stands for 2^(byte - 127), 255 for NaN.
  *          Bytes of a tile that belong to no row or block are 0.
- * Both 16-byte aligned. */
+ * Both 16-byte aligned.  The functions' outputs overlap none of their inputs. */
 
 /* Quantises x [rows, cols] (row stride x_stride elements; fp32, fp16 or bf16)
  * along its rows: scale 2^(floor(log2 max|x|) - 2) per block (clamped to the
@@ -410,7 +410,8 @@ AOTK_API int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, const
  * scale, in one pass (all [rows, cols], one dtype, fp32 math):
  *   h_out = residual_scale * residual + gate * rms(x) * post_weight
  *   out   = rms(h) * pre_weight, rms(v) = v * rsqrt(mean(v^2) + eps)
- * out is computed from the unrounded h.  gate (may be null) is [gate_rows,
+ * out is computed from the unrounded h.  out and h_out overlap no input (rows
+ * are read ahead).  gate (may be null) is [gate_rows,
  * gate_cols]: gate_cols is cols or 1, gate_rows divides rows, and row r uses
  * gate row r / (rows / gate_rows).  No reference counterpart: the reference
  * composes its rmsnorm (aot_kernel/norm.py:9-18) with torch. */
