@@ -410,7 +410,8 @@ AOTK_API int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, const
  * scale, in one pass (all [rows, cols], one dtype, fp32 math):
  *   h_out = residual_scale * residual + gate * rms(x) * post_weight
  *   out   = rms(h) * pre_weight, rms(v) = v * rsqrt(mean(v^2) + eps)
- * out is computed from the unrounded h.  out and h_out overlap no input (rows
+ * out is computed from the unrounded h.  Rows of any finite values are
+ * normalised, whether or not their squares fit fp32.  out and h_out overlap no input (rows
  * are read ahead).  gate (may be null) is [gate_rows,
  * gate_cols]: gate_cols is cols or 1, gate_rows divides rows, and row r uses
  * gate row r / (rows / gate_rows).  No reference counterpart: the reference

@@ -57,7 +57,8 @@ def sandwich_rmsnorm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch
     x: its last dim is H or 1, its leading dims match x's from the left and are 1
     after that - e.g. ``[H]`` (per channel), ``[B, 1, H]`` (per sequence),
     ``[B, S, 1]`` (per token) or x's own shape.  A factor on the block's branch
-    can be folded into ``gate`` or ``post_weight``.  All tensors are contiguous and of
+    can be folded into ``gate`` or ``post_weight``.  Rows of any finite values are
+    normalised, whether or not their squares fit fp32.  All tensors are contiguous and of
     one dtype; anything else is a ValueError.  Forward only, like the other norms.
     """
     if not x.is_cuda:

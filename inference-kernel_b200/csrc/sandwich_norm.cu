@@ -16,6 +16,11 @@
 //   * sandwich_long_kernel: rows that fit neither, or tensors that do not start
 //     on 16 bytes: the row is read three times.
 //
+// Squares of bf16's and fp32's largest numbers (from about 1.8e19 on) and, with a
+// small eps, of their smallest leave fp32's range, where rms(v) itself is of order 1.
+// Rows whose mean square shows that are computed again (row_out_of_range); the others
+// pay a few comparisons.
+//
 // gate is [gate_rows, gate_cols]: gate_cols is the row length or 1, and row r
 // of the problem uses gate row r / (rows / gate_rows) - one row for all
 // (per channel), one for each sequence, or one for each token.
@@ -67,6 +72,98 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
     for (int k = 0; k < WPR; ++k) v += buf[first + k];
   }
   return v;
+}
+
+// The lanes of this thread's row in its warp.
+template <int TPR>
+__device__ __forceinline__ unsigned row_lanes() {
+  if constexpr (TPR >= 32) return 0xffffffffu;
+  return ((1u << (TPR & 31)) - 1) << (threadIdx.x & 31 & ~(TPR - 1));
+}
+
+// Waits for the threads of a row; `group` numbers the rows of a block.
+template <int TPR>
+__device__ __forceinline__ void group_sync(int group) {
+  if constexpr (TPR <= 32)
+    __syncwarp(row_lanes<TPR>());
+  else
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+}
+
+// m = mean(v^2) + eps of a row.  Below 2^-100 squares may have been lost (one that is
+// keeps an error of 2^-150 at most, 2^-50 of such a mean); infinity says that the sum
+// overflowed, unless v holds one.  NaN counts as out of range, and stays NaN.
+__device__ __forceinline__ bool out_of_range(float m) {
+  constexpr uint32_t kLow = 27u << 23, kTop = 0x7F7FFFFFu;  // 2^-100, the largest number
+  return __float_as_uint(m) - kLow > kTop - kLow;
+}
+
+// A row with such a mean square, of x or of h, once more, element by element from its
+// inputs: v is multiplied by f = 2^96 or 2^-96 before it is squared, so that |f v| <= 2^32,
+// or |f v| < 2^62 (a mean below 2^-100 leaves |v| < 2^-50 sqrt(cols)) with no number below
+// 2^-53, and what counts fits.  v / rms is (v f) inv for small numbers and (v inv) f for
+// large ones, so that neither step takes bits from a number that is small beside its row.
+// Called by the TPR threads of the row, `t` of them, with `buf` for their warps' sums;
+// writes after what they wrote before.
+template <typename T, int TPR>
+__device__ __forceinline__ void row_out_of_range(const Args<T>& a, int64_t row, int t, int group,
+                                                 float* buf) {
+  const int n = a.cols;
+  const int64_t off = row * n;
+  group_sync<TPR>(group);
+  auto row_sum_of = [&](auto v_at, float f) {
+    float s = 0.f;
+#pragma unroll 1
+    for (int c = t; c < n; c += TPR) {
+      const float v = v_at(c) * f;
+      s = fmaf(v, v, s);
+    }
+#pragma unroll
+    for (int o = TPR < 32 ? TPR / 2 : 16; o > 0; o >>= 1) s += __shfl_xor_sync(row_lanes<TPR>(), s, o);
+    if constexpr (TPR > 32) {
+      group_sync<TPR>(group);  // all have read buf
+      if ((t & 31) == 0) buf[t / 32] = s;
+      group_sync<TPR>(group);
+      s = 0.f;
+#pragma unroll 1
+      for (int k = 0; k < TPR / 32; ++k) s += buf[k];
+    }
+    return s;
+  };
+  struct TwoSteps {
+    float first, second;
+  };
+  auto inverse = [&](auto v_at) {
+    const float cols = static_cast<float>(a.cols);
+    const float m = row_sum_of(v_at, 1.f) / cols + a.eps;
+    const float f = !out_of_range(m) ? 1.f : m < 1.f ? 0x1p96f : 0x1p-96f;
+    const float inv = rsqrtf(row_sum_of(v_at, f) / cols + a.eps * f * f);
+    return m < 1.f ? TwoSteps{f, inv} : TwoSteps{inv, f};
+  };
+  const T* gate = static_cast<const T*>(a.gate.ptr);
+  if (gate != nullptr) gate += row / a.gate.rows_per * a.gate.row_stride;
+  auto x_at = [&](int c) { return Elem<T>::to_f(a.x[off + c]); };
+  const TwoSteps by_x = inverse(x_at);
+  auto h_at = [&](int c) {
+    float v = x_at(c) * by_x.first * by_x.second * Elem<T>::to_f(a.post[c]);
+    if (gate != nullptr) v *= Elem<T>::to_f(gate[a.gate.col_stride ? c : 0]);
+    return fmaf(a.alpha, Elem<T>::to_f(a.residual[off + c]), v);
+  };
+  const TwoSteps by_h = inverse(h_at);
+#pragma unroll 1
+  for (int c = t; c < n; c += TPR) {
+    const float h = h_at(c);
+    a.h_out[off + c] = Elem<T>::from_f(h);
+    a.out[off + c] = Elem<T>::from_f(h * by_h.first * by_h.second * Elem<T>::to_f(a.pre[c]));
+  }
+}
+
+// The same out of line, for rows of a warp or less, of which there may be many at a time:
+// inlined it costs their kernels registers, and with them blocks per SM (16384 x 256 bf16
+// 7.7 us; inline 9.9).
+template <typename T, int TPR>
+__device__ __noinline__ void row_out_of_range_call(const Args<T>& a, int64_t row, int t, int group) {
+  row_out_of_range<T, TPR>(a, row, t, group, nullptr);
 }
 
 // Elements [pos + lo, pos + hi) of `base` in their places of a vector, one by one.
@@ -178,12 +275,25 @@ struct ShiftedWeight {
 
 constexpr int threads_for(int tpr) { return tpr > 256 ? tpr : 256; }
 
+// Blocks per SM that rows of a warp or less are compiled for, one of which the registers
+// of the call behind them would cost (65536 x 128 bf16 13.2 us; 16.9 with three blocks).
+// Unaligned 16-bit rows of two vectors keep theirs, and lose if held to it (30000 x 99 fp16
+// 11.3 -> 12.0).
+template <typename T, bool kShift, int VPT, int TPR>
+constexpr int blocks_for() {
+  constexpr bool kWide = kShift && std::is_same_v<T, __nv_bfloat16>;
+  if (TPR > 32) return 1;
+  if (VPT == 1) return kWide ? 4 : 5;
+  return kShift && sizeof(T) == 2 ? 1 : 4;
+}
+
 // kShift: rows need not start on 16 bytes (the tensors do).  A thread's vectors
 // are those of the tensors, so the row's first and last may hold elements of its
 // neighbours, which count as zeros and are not written; the weights' elements are
 // shifted into the places of the row's.
 template <typename T, bool kShift, int VPT, int TPR>
-__global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T> a) {
+__global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, TPR>())
+    sandwich_kernel(const __grid_constant__ Args<T> a) {
   constexpr int E = Elem<T>::kPerVec;
   constexpr int P = E / 2;  // pairs per vector
   constexpr int kThreads = threads_for(TPR);
@@ -306,7 +416,8 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
     }
   }
   const float sum = row_sum<TPR>(ss.x + ss.y, buf[0]);
-  const float inv = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+  const float mean = sum / static_cast<float>(a.cols) + a.eps;
+  const float inv = rsqrtf(mean);
 
   ss = make_float2(0.f, 0.f);
   const float scale = inv * g_row;
@@ -334,7 +445,8 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
     }
   }
   const float sum_h = row_sum<TPR>(ss.x + ss.y, buf[1]);
-  const float inv_h = rsqrtf(sum_h / static_cast<float>(a.cols) + a.eps);
+  const float mean_h = sum_h / static_cast<float>(a.cols) + a.eps;
+  const float inv_h = rsqrtf(mean_h);
   const float2 inv_h2 = make_float2(inv_h, inv_h);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -346,6 +458,14 @@ __global__ void __launch_bounds__(threads_for(TPR)) sandwich_kernel(const Args<T
       for (int e = 0; e < P; ++e) w[e] = mul2(mul2(h[i][e], inv_h2), w[e]);
       write(a.out, column(i), w);
     }
+  }
+  // The row's threads have the same sums.
+  if (live && (out_of_range(mean) | out_of_range(mean_h))) {
+    const int group = threadIdx.x / TPR;
+    if constexpr (TPR <= 32)
+      row_out_of_range_call<T, TPR>(a, row, t, group);
+    else
+      row_out_of_range<T, TPR>(a, row, t, group, buf[0] + group * (TPR / 32));
   }
 }
 
@@ -392,14 +512,6 @@ __device__ __forceinline__ float group_sum(float v, float* buf, int group, int t
     for (int k = 0; k < TPR / 32; ++k) v += buf[k];
   }
   return v;
-}
-
-template <int TPR>
-__device__ __forceinline__ void group_sync(int group) {
-  if constexpr (TPR == 32)
-    __syncwarp();
-  else
-    asm volatile("barrier.cta.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
 }
 
 // kShift: rows need not start on 16 bytes (the tensors do).  The copies take the
@@ -524,6 +636,15 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     }
   }
 
+  // Rows out of range are written as NaN, and again once the group has no more rows to
+  // stream: what that needs is not held meanwhile.
+  bool again = false;
+  auto inverse = [&](float sum) {
+    const float mean = sum / static_cast<float>(a.cols) + a.eps;
+    const bool out = out_of_range(mean);
+    again |= out;
+    return out ? __int_as_float(0x7fc00000) : rsqrtf(mean);
+  };
   int stage = 0;
   uint32_t phase = 0;
   for (int64_t row = first_row; row < a.rows; row += step) {
@@ -599,9 +720,9 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         const bool wraps = stage + k >= stages;
         mbar_drain(bar0 + 8u * (stage + k - (wraps ? stages : 0)), phase ^ (wraps ? 1u : 0u));
       }
-      break;
+      return;
     }
-    const float inv = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+    const float inv = inverse(sum);
 
     ss = make_float2(0.f, 0.f);
     const float scale = gate_cols ? inv : inv * g_row;
@@ -630,7 +751,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     const float sum_h = group_sum<TPR>(ss.x + ss.y, partial[group][1], group, t, bad);
     // The whole group has read the stage.
     if (t == 0 && row + stages * step < a.rows) request(row + stages * step, stage);
-    const float inv_h = rsqrtf(sum_h / static_cast<float>(a.cols) + a.eps);
+    const float inv_h = inverse(sum_h);
     const float2 inv_h2 = make_float2(inv_h, inv_h);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -651,6 +772,14 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     if (++stage == stages) {
       stage = 0;
       phase ^= 1u;
+    }
+  }
+  if (again) {  // the whole group: its threads have the same sums
+    group_sync<TPR>(group);
+    for (int64_t row = first_row; row < a.rows; row += step) {
+      const T* first = a.out + row * a.cols;
+      if (isnan(Elem<T>::to_f(*first)))  // what the group wrote, or NaN by the formula
+        row_out_of_range<T, TPR>(a, row, t, group, partial[group][0]);
     }
   }
 }
@@ -687,7 +816,8 @@ __global__ void __launch_bounds__(kLongThreads) sandwich_long_kernel(const Args<
     for (int e = 0; e < E; ++e) ss = fmaf(f[e], f[e], ss);
   }
   ss = row_sum<kLongThreads>(ss, buf[0]);
-  const float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  const float mean = ss / static_cast<float>(a.cols) + a.eps;
+  const float inv = rsqrtf(mean);
   const T* gate = static_cast<const T*>(a.gate.ptr);
   if (gate != nullptr) gate += row / a.gate.rows_per * a.gate.row_stride;
   const bool gate_cols = gate != nullptr && a.gate.col_stride;
@@ -715,7 +845,12 @@ __global__ void __launch_bounds__(kLongThreads) sandwich_long_kernel(const Args<
     for (int e = 0; e < E; ++e) ss = fmaf(h[e], h[e], ss);
   }
   ss = row_sum<kLongThreads>(ss, buf[1]);
-  const float inv_h = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  const float mean_h = ss / static_cast<float>(a.cols) + a.eps;
+  if (out_of_range(mean) || out_of_range(mean_h)) {
+    row_out_of_range<T, kLongThreads>(a, row, threadIdx.x, 0, buf[0]);
+    return;
+  }
+  const float inv_h = rsqrtf(mean_h);
   for (int64_t c = threadIdx.x * E; c < a.cols; c += step) {
     float h[E], w[E];
     h_at(c, h);
