@@ -338,8 +338,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    // The first CTA's full barriers see every load: drain there.
-    if (elected && rank == 0) {
+    // The first CTA's full barriers see every load: drain there.  The second is sent
+    // commits, and does not leave before the last of them have arrived (those of tfull
+    // are the epilogue's).
+    if (elected) {
       int s = stage;
       uint32_t p = phase;
       for (int i = 0; i < stages && i < issued; ++i) {
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           s = stages - 1;
           p ^= 1u;
         }
-        mbar_drain(full_bar(s), p);
+        if (!mbar_drain(rank == 0 ? full_bar(s) : empty_bar(s), p) && rank != 0) break;
       }
     }
     __syncwarp();
@@ -435,8 +437,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       if (elected) {
-        commit(drain_bar);
+        if constexpr (CG == 2)
+          umma_commit_pair(drain_bar, 0x1);
+        else
+          umma_commit(drain_bar);
         mbar_drain(drain_bar, 0);
+        // The second CTA signals its last read-outs here, and no further tile waits for
+        // them: the cluster's barriers are relaxed, so that they do not show it either.
+        if constexpr (CG == 2)
+          for (int i = it > L::kAccs ? it - L::kAccs : 0; i < it; ++i)
+            if (!mbar_drain(release_bar(i % L::kAccs), (i / L::kAccs) & 1)) break;
       }
     }
     __syncwarp();

@@ -241,17 +241,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // The first CTA's full barriers see every load of the pair: drain there.
-      if (rank == 0) {
-        int s = stage;
-        uint32_t p = phase;
-        for (int i = 0; i < STAGES && i < issued; ++i) {
-          if (--s < 0) {
-            s = STAGES - 1;
-            p ^= 1u;
-          }
-          mbar_drain(full_bar(s), p);
+      // The first CTA's full barriers see every load of the pair: drain there.  The
+      // second is sent commits, and does not leave before the last of them have
+      // arrived (those of tfull are the epilogue's).
+      int s = stage;
+      uint32_t p = phase;
+      for (int i = 0; i < STAGES && i < issued; ++i) {
+        if (--s < 0) {
+          s = STAGES - 1;
+          p ^= 1u;
         }
+        if (!mbar_drain(rank == 0 ? full_bar(s) : empty_bar(s), p) && rank != 0) break;
       }
     }
     __syncwarp();
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           acc_phase ^= 1u;
         }
       }
-      umma_commit_pair(drain_bar, 0x3);
+      umma_commit_pair(drain_bar, 0x1);
       mbar_drain(drain_bar, 0);
     }
     __syncwarp();
