@@ -34,8 +34,8 @@ struct ReluOp {
 
 // Unary map over n_vec 16-byte vectors.
 template <typename T, typename Op>
-__global__ void __launch_bounds__(kThreads) unary_vec_kernel(const uint4* __restrict__ x,
-                                                             uint4* __restrict__ y, int64_t n_vec) {
+__global__ void __launch_bounds__(kThreads) unary_vec_kernel(const uint4* x, uint4* __restrict__ y,
+                                                             int64_t n_vec) {
   constexpr int E = Elem<T>::kPerVec;
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
@@ -64,8 +64,7 @@ __global__ void __launch_bounds__(kThreads) unary_vec_kernel(const uint4* __rest
 
 // Scalar remainder / unaligned fallback.
 template <typename T, typename Op>
-__global__ void __launch_bounds__(kThreads) unary_scalar_kernel(const T* __restrict__ x,
-                                                                T* __restrict__ y, int64_t n) {
+__global__ void __launch_bounds__(kThreads) unary_scalar_kernel(const T* x, T* __restrict__ y, int64_t n) {
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
   const int64_t step = (int64_t)gridDim.x * kThreads;
@@ -78,7 +77,7 @@ __global__ void __launch_bounds__(kThreads) unary_scalar_kernel(const T* __restr
 // vectorised along the row when every row start is 16-byte aligned.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) silu_mul_vec_kernel(
-    const T* __restrict__ gate, int64_t gate_stride, const T* __restrict__ up, int64_t up_stride,
+    const T* gate, int64_t gate_stride, const T* up, int64_t up_stride,
     T* __restrict__ out, int64_t out_stride, int64_t rows, int64_t vec_per_row) {
   constexpr int E = Elem<T>::kPerVec;
   const int64_t n_vec = rows * vec_per_row;
@@ -117,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) silu_mul_vec_kernel(
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) silu_mul_scalar_kernel(
-    const T* __restrict__ gate, int64_t gate_stride, const T* __restrict__ up, int64_t up_stride,
+    const T* gate, int64_t gate_stride, const T* up, int64_t up_stride,
     T* __restrict__ out, int64_t out_stride, int64_t rows, int64_t cols) {
   const int64_t n = rows * cols;
   sm100::pdl_launch_dependents();

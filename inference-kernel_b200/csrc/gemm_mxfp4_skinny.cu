@@ -85,9 +85,8 @@ template <typename T, int MP, int STAGES, int SEGS, bool kAlias>
 __global__ void __launch_bounds__(kThreads, 2)
     gemm_mxfp4_skinny_kernel(const __grid_constant__ CUtensorMap tmW,
                              const __grid_constant__ CUtensorMap tmX,
-                             const uint8_t* __restrict__ w_scales,
-                             const uint8_t* __restrict__ x_scales, T* __restrict__ c, int M, int N,
-                             int K, int strips_per_cluster) {
+                             const uint8_t* w_scales, const uint8_t* x_scales,
+                             T* __restrict__ c, int M, int N, int K, int strips_per_cluster) {
   using L = MxsLayout<MP, STAGES, SEGS, kAlias>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);

@@ -379,11 +379,11 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
 // Columns at or beyond n read as 0; n % 4 == 0, so a group is all in or out.
 __device__ __forceinline__ float4 load_sb4(const ScaleParams& sc, int col, int n) {
   if (sc.sb_step == 0) {
-    const float v = __ldg(sc.sb);
+    const float v = *sc.sb;
     return make_float4(v, v, v, v);
   }
   if (col >= n) return make_float4(0.f, 0.f, 0.f, 0.f);
-  return __ldg(reinterpret_cast<const float4*>(sc.sb + col));
+  return *reinterpret_cast<const float4*>(sc.sb + col);
 }
 
 template <typename Op, typename T, int BN, int STAGES, int kEpi>
@@ -754,7 +754,7 @@ __global__ void __launch_bounds__(kEpi == kEpiAllReduce ? kThreadsFused : kThrea
             // Row scale (an rms_norm rstd folded out of A): gate and up
             // accumulators are both linear in the row.
             const int row = mb * kBM + row_in_tile;
-            const float rs = row < M ? __ldg(sc.sa + row) : 0.f;
+            const float rs = row < M ? sc.sa[row] : 0.f;
 #pragma unroll
             for (int j = 0; j < 64; ++j) {
               g[j] *= rs;
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kEpi == kEpiAllReduce ? kThreadsFused : kThrea
         if (store_x >= N || store_y >= M) continue;  // box entirely outside C
         if constexpr (kScaled) {
           const int row = mb * kBM + row_in_tile;
-          const float sa = row < M ? __ldg(sc.sa + static_cast<size_t>(row) * sc.sa_step) : 0.f;
+          const float sa = row < M ? sc.sa[static_cast<size_t>(row) * sc.sa_step] : 0.f;
 #pragma unroll
           for (int j = 0; j < 64; j += 4) {
             const float4 sb = load_sb4(sc, store_x + j, N);

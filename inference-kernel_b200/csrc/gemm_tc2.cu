@@ -118,7 +118,7 @@ template <typename T, int STAGES, int BNP, bool kSiluMul>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, int M, int N, int K, uint32_t idesc,
-                    const float* __restrict__ row_scale, int tail_begin) {
+                    const float* row_scale, int tail_begin) {
   using L = Tc2Layout<STAGES, BNP>;
   constexpr int kBN = BNP;
   const int n_out = kSiluMul ? N / 2 : N;  // columns of the output
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           half >= 0 ? (kSiluMul ? kBN / 256 : kBN / 128) : (kSiluMul ? kBN / 128 : kBN / 64);
       const int row = store_y + lane;
       float rs = 1.f;
-      if (kSiluMul && row_scale != nullptr) rs = row < M ? __ldg(row_scale + row) : 0.f;
+      if (kSiluMul && row_scale != nullptr) rs = row < M ? row_scale[row] : 0.f;
 #pragma unroll 1
       for (int c = 0; c < out_chunks; ++c) {
         float f[64];

@@ -176,8 +176,8 @@ struct Block {
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                    const T* __restrict__ x, int64_t stride, int64_t rows, int64_t rows_padded,
-                    int cols, const Walk walk) {
+                    const T* x, int64_t stride, int64_t rows, int64_t rows_padded, int cols,
+                    const Walk walk) {
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();
   int64_t row;
@@ -229,8 +229,8 @@ constexpr int kOutUnroll = 2;
 
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
-    dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes,
-                      const uint8_t* __restrict__ scales, int64_t rows, int cols, const Walk walk) {
+    dequantize_kernel(T* __restrict__ out, const uint8_t* codes, const uint8_t* scales,
+                      int64_t rows, int cols, const Walk walk) {
   constexpr int E = kOutItem<T>, U = kOutUnroll;
   sm100::pdl_launch_dependents();
   sm100::pdl_wait_prior();

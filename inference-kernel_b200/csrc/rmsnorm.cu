@@ -25,7 +25,7 @@ namespace {
 constexpr int kBlock = 256;
 
 template <typename T, int VPT, int TPR>
-__device__ __forceinline__ void load_row(const T* __restrict__ x, int64_t row, int64_t rows,
+__device__ __forceinline__ void load_row(const T* x, int64_t row, int64_t rows,
                                          int cols, int t, uint4 (&v)[VPT]) {
   constexpr int E = Elem<T>::kPerVec;
   const int n_vec = cols / E;
@@ -48,9 +48,9 @@ __device__ __forceinline__ void load_row(const T* __restrict__ x, int64_t row, i
 // `stats`) and no normalised row.
 template <typename T, int VPT, int TPR, bool kRes, bool kStats = false>
 __global__ void __launch_bounds__(TPR > kBlock ? TPR : kBlock)
-    rmsnorm_vec_kernel(const T* __restrict__ x, const T* __restrict__ res, const T* __restrict__ w,
-                       T* __restrict__ y, T* __restrict__ h_out, int64_t rows, int cols,
-                       float eps, float* __restrict__ stats = nullptr) {
+    rmsnorm_vec_kernel(const T* x, const T* res, const T* w, T* __restrict__ y,
+                       T* __restrict__ h_out, int64_t rows, int cols, float eps,
+                       float* __restrict__ stats = nullptr) {
   constexpr int E = Elem<T>::kPerVec;
   constexpr int THREADS = TPR > kBlock ? TPR : kBlock;
   constexpr int RPB = THREADS / TPR;  // rows per block

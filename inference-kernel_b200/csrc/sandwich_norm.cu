@@ -300,6 +300,9 @@ __global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, T
   constexpr int RPB = kThreads / TPR;
   // With 1024 threads the registers hold the row, but not its weights too.
   constexpr bool kEarly = TPR < 1024;
+  // Nor do the 64 that leave room for four blocks per SM: there the second weight comes
+  // after the first sum (65536 x 128 bf16 13.1 us; 16.6 with spills).
+  constexpr bool kPreLate = TPR <= 32 && std::is_same_v<T, __nv_bfloat16> && !kShift && VPT == 2;
   __shared__ float buf[2][kThreads / 32];
   const int t = threadIdx.x % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
@@ -398,7 +401,7 @@ __global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, T
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
         load_post(i);
-        load_pre(i);
+        if constexpr (!kPreLate) load_pre(i);
       }
     }
   }
@@ -418,6 +421,12 @@ __global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, T
   const float sum = row_sum<TPR>(ss.x + ss.y, buf[0]);
   const float mean = sum / static_cast<float>(a.cols) + a.eps;
   const float inv = rsqrtf(mean);
+
+  if constexpr (kPreLate) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (used(i)) load_pre(i);
+  }
 
   ss = make_float2(0.f, 0.f);
   const float scale = inv * g_row;
@@ -611,16 +620,19 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   // A thread's columns are the same in every row, so their weights stay in
   // registers (from L2 they would be as many bytes per row as x and the residual),
   // and so does the gate until its row changes.  Weights of more than four vectors do
-  // not fit there and are read again for every row, which is still better than a row
-  // at a time in the registers of 1024 threads (1024 x 20480 bf16 56 -> 32 us).
+  // not fit there and are read again for every row, ahead of the sum before their use,
+  // which is still better than a row at a time in the registers of 1024 threads
+  // (1024 x 20480 bf16 56 -> 28 us).
   constexpr bool kKeep = VPT <= 4;
   static_assert(kKeep || !kShift, "shifted once");
-  uint4 post[kKeep ? VPT : 1], pre[kKeep ? VPT : 1], g[VPT];
-  auto weight = [&](const uint4* kept, const T* w, int i) {
-    if constexpr (kKeep)
-      return kept[i];
-    else
-      return ld_cached(reinterpret_cast<const uint4*>(w) + t + i * TPR);
+  uint4 post[kKeep ? VPT : 1], pre[kKeep ? VPT : 1], g[VPT], reread[kKeep ? 1 : VPT];
+  auto weight = [&](const uint4* kept, int i) { return kKeep ? kept[i] : reread[kKeep ? 0 : i]; };
+  auto read_weight = [&](const T* w) {
+    if constexpr (!kKeep) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (used(i)) reread[i] = ld_cached(reinterpret_cast<const uint4*>(w) + t + i * TPR);
+    }
   };
   float g_row = 1.f;
   int64_t g_at = 0, g_end = 0;  // the gate row in use, the first row beyond it
@@ -714,6 +726,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         for (int e = 0; e < P; ++e) ss = fma2(h[i][e], h[i][e], ss);
       }
     }
+    read_weight(a.post);
     const float sum = group_sum<TPR>(ss.x + ss.y, partial[group][0], group, t, bad);
     if (bad) {  // the whole group, once what it has requested has arrived
       for (int k = 0; t == 0 && k < stages && row + k * step < a.rows; ++k) {
@@ -731,7 +744,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(weight(post, a.post, i), &w[0].x);
+        Elem<T>::unpack(weight(post, i), &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) h[i][e] = mul2(mul2(h[i][e], scale2), w[e]);
         if (gate_cols) {
@@ -748,6 +761,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         write(a.h_out, 0, i, h[i]);
       }
     }
+    read_weight(a.pre);
     const float sum_h = group_sum<TPR>(ss.x + ss.y, partial[group][1], group, t, bad);
     // The whole group has read the stage.
     if (t == 0 && row + stages * step < a.rows) request(row + stages * step, stage);
@@ -757,7 +771,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (int i = 0; i < VPT; ++i) {
       if (used(i)) {
         float2 w[P];
-        Elem<T>::unpack(weight(pre, a.pre, i), &w[0].x);
+        Elem<T>::unpack(weight(pre, i), &w[0].x);
 #pragma unroll
         for (int e = 0; e < P; ++e) w[e] = mul2(mul2(h[i][e], inv_h2), w[e]);
         write(a.out, 1, i, w);

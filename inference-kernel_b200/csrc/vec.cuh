@@ -9,23 +9,31 @@
 
 namespace aotk {
 
-// Read-only 16-byte load that bypasses L1 allocation (each byte is read once).
+// Loads of inputs.  Kernels of dependent launches start while the kernel that writes
+// their inputs may still run, so an input is not read-only as long as they run: no load
+// is of the read-only kind (ld.global.nc, which the compiler also takes for `const
+// __restrict__` parameters and may move above pdl_wait_prior()).  Plain loads stay behind
+// the wait and its memory clobber, and volatile statements behind each other; a load in a
+// statement that is not volatile could be executed ahead of the condition that guards it.
+// Neither kind runs ahead of an earlier store, so loads are written where they should start.
+
+// 16-byte load that bypasses L1 allocation (each byte is read once).
 __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
 }
 
 // 16-byte load through L1 (for data reused by several warps, e.g. norm weights).
-__device__ __forceinline__ uint4 ld_cached(const uint4* p) { return __ldg(p); }
+__device__ __forceinline__ uint4 ld_cached(const uint4* p) { return *p; }
 
-// Read-only 32-byte load (32-byte aligned) that bypasses L1 allocation: a lane's
+// 32-byte load (32-byte aligned) that bypasses L1 allocation: a lane's
 // two vectors as one request, where two 16-byte loads would fetch each 32-byte
 // sector twice.
 __device__ __forceinline__ void ld_stream32(const void* p, uint4& a, uint4& b) {
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z),
                  "=r"(b.w)
                : "l"(p));
