@@ -12,10 +12,9 @@
 // griddepcontrol.wait, so its own launch and setup overlap the tail of the
 // kernel before it.
 #include "common.h"
+#include "host_cache.h"
 #include "sm100.cuh"
 #include "vec.cuh"
-
-#include <mutex>
 
 namespace aotk {
 namespace {
@@ -134,21 +133,14 @@ __global__ void __launch_bounds__(kThreads) silu_mul_scalar_kernel(
 // Blocks of `kernel` that are resident at once on one SM of the current
 // device (cached per kernel and device; at most kBlocksPerSm).
 int resident_per_sm(const void* kernel, const DeviceInfo& info) {
-  struct Entry {
-    const void* kernel;
-    int device, n;
-  };
-  static std::mutex mu;
-  static Entry cache[64];
-  static int count = 0;
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < count; ++i)
-    if (cache[i].kernel == kernel && cache[i].device == info.device) return cache[i].n;
-  int n = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, 0) != cudaSuccess || n < 1)
-    n = 1;
-  if (n > kBlocksPerSm) n = kBlocksPerSm;
-  if (count < 64) cache[count++] = Entry{kernel, info.device, n};
+  static DeviceCache<64> cache;
+  int n = 1;
+  cache.get(info.device, reinterpret_cast<uintptr_t>(kernel), &n, [&](int* v) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(v, kernel, kThreads, 0) != cudaSuccess || *v < 1)
+      *v = 1;
+    if (*v > kBlocksPerSm) *v = kBlocksPerSm;
+    return 0;
+  });
   return n;
 }
 

@@ -3,12 +3,13 @@
 
 #include <mutex>
 
+#include "host_cache.h"
+
 namespace aotk {
 
 namespace {
 thread_local char g_last_error[512] = "no error";
 
-constexpr int kMaxDevices = 64;
 DeviceInfo g_info[kMaxDevices];
 std::once_flag g_info_once[kMaxDevices];
 }  // namespace

@@ -17,23 +17,13 @@
 // (aot_kernel/gemm.py:39-42).
 #include <cuda_runtime.h>
 
-#include <mutex>
-
 #include "common.h"
 #include "gemm_internal.h"
+#include "host_cache.h"
 
 namespace aotk {
 
 namespace {
-
-struct SmemKey {
-  const void* kernel;
-  int device;
-};
-
-std::mutex g_smem_mu;
-SmemKey g_smem_done[256];
-int g_smem_count = 0;
 
 int validate_common(const char* who, const void* c, const void* a, const void* b, int64_t M,
                     int64_t N, int64_t K, int dtype) {
@@ -57,18 +47,18 @@ int zero_output(void* c, int64_t M, int64_t N, int dtype, void* stream) {
 }  // namespace
 
 int ensure_dynamic_smem(const void* kernel, int bytes, const DeviceInfo& info) {
-  std::lock_guard<std::mutex> lock(g_smem_mu);
-  for (int i = 0; i < g_smem_count; ++i) {
-    if (g_smem_done[i].kernel == kernel && g_smem_done[i].device == info.device) return AOTK_OK;
-  }
-  if (bytes > info.max_smem_optin)
-    return fail(AOTK_ERR_DEVICE, "kernel needs %d bytes of shared memory, device allows %d", bytes,
-                info.max_smem_optin);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess)
-    return fail(AOTK_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", bytes, cudaGetErrorString(e));
-  if (g_smem_count < 256) g_smem_done[g_smem_count++] = SmemKey{kernel, info.device};
-  return AOTK_OK;
+  static DeviceCache<1024> done;
+  int limit;
+  return done.get(info.device, reinterpret_cast<uintptr_t>(kernel), &limit, [&](int* v) -> int {
+    if (bytes > info.max_smem_optin)
+      return fail(AOTK_ERR_DEVICE, "kernel needs %d bytes of shared memory, device allows %d", bytes,
+                  info.max_smem_optin);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess)
+      return fail(AOTK_ERR_CUDA, "cudaFuncSetAttribute(smem=%d): %s", bytes, cudaGetErrorString(e));
+    *v = bytes;
+    return AOTK_OK;
+  });
 }
 
 bool tc_eligible(const void* c, const void* a, const void* b, int64_t M, int64_t N, int64_t K,

@@ -22,11 +22,10 @@
 // 128-row tile (aot_kernel/csrc/gemm/gemm_opt.cu:174-192).
 #include "common.h"
 #include "gemm_internal.h"
+#include "host_cache.h"
 #include "sm100.cuh"
 #include "tmap.h"
 #include "vec.cuh"
-
-#include <mutex>
 
 namespace aotk {
 namespace {
@@ -243,10 +242,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// A kernel with the skinny kernel's block shape and no TMEM, used only for
+// A kernel with the skinny kernels' block shape and no TMEM, used only for
 // occupancy queries: the driver reports one block per SM for any kernel that
 // allocates TMEM (it cannot know how many columns each CTA takes), while two
-// skinny CTAs - at most 128 + 128 of the 512 columns - do run side by side on
+// skinny CTAs - at most 256 + 256 of the 512 columns - do run side by side on
 // an SM when shared memory allows, and clusters pack accordingly.
 __global__ void __launch_bounds__(kThreads, 2) skinny_shadow_kernel() {}
 
@@ -255,43 +254,31 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_shadow_kernel() {}
 // Clusters of `cs` skinny CTAs with `smem` bytes each that can be resident at
 // once on the device (cached per device, cluster size and shared-memory size).
 int resident_clusters(int cs, int smem, const DeviceInfo& info, int* out) {
-  struct Entry {
-    int device, cs, smem, n;
-  };
-  static std::mutex mu;
-  static Entry cache[64];
-  static int count = 0;
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < count; ++i) {
-    if (cache[i].device == info.device && cache[i].cs == cs && cache[i].smem == smem) {
-      *out = cache[i].n;
-      return AOTK_OK;
-    }
-  }
-  // The limit is set once per kernel and device, so to the most that any caller
-  // may ask for: a query above a smaller limit finds no room for any cluster.
-  if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(skinny_shadow_kernel),
-                                   info.max_smem_optin, info))
-    return st;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(cs), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cs);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  cudaError_t e = cudaOccupancyMaxActiveClusters(&n, skinny_shadow_kernel, &cfg);
-  if (e != cudaSuccess)
-    return fail(AOTK_ERR_CUDA, "skinny gemm: cluster occupancy (size %d): %s", cs,
-                cudaGetErrorString(e));
-  if (count < 64) cache[count++] = Entry{info.device, cs, smem, n};
-  *out = n;
-  return AOTK_OK;
+  static DeviceCache<256> cache;
+  const uint64_t key = static_cast<uint64_t>(smem) << 8 | static_cast<uint64_t>(cs);
+  return cache.get(info.device, key, out, [&](int* n) -> int {
+    // The limit is set once per kernel and device, so to the most that any caller
+    // may ask for: a query above a smaller limit finds no room for any cluster.
+    if (int st = ensure_dynamic_smem(reinterpret_cast<const void*>(skinny_shadow_kernel),
+                                     info.max_smem_optin, info))
+      return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(cs), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(cs);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaOccupancyMaxActiveClusters(n, skinny_shadow_kernel, &cfg);
+    if (e != cudaSuccess)
+      return fail(AOTK_ERR_CUDA, "skinny gemm: cluster occupancy (size %d): %s", cs,
+                  cudaGetErrorString(e));
+    return AOTK_OK;
+  });
 }
 
 namespace {
