@@ -406,6 +406,18 @@ AOTK_API int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, const
                              const void* b_scales, int64_t M, int64_t N, int64_t K, int out_dtype,
                              void* stream);
 
+enum {
+  AOTK_MXFP4_SPLIT = 0,    /* K split over clusters, two CTAs per SM (M <= 128) */
+  AOTK_MXFP4_PAIR_256 = 1, /* 256 x 256 tiles on CTA pairs */
+  AOTK_MXFP4_PAIR_128 = 2, /* 256 x 128 tiles on CTA pairs */
+  AOTK_MXFP4_ONE_128 = 3,  /* 128 x 128 tiles on one CTA */
+  AOTK_MXFP4_ONE_64 = 4    /* 128 x 64 tiles on one CTA */
+};
+
+/* The kernel aotk_mxfp4_gemm runs for a problem on a device with `sm_count`
+ * SMs.  Pure host arithmetic.  No reference counterpart. */
+AOTK_API int aotk_mxfp4_gemm_path(int64_t M, int64_t N, int64_t K, int sm_count, int* path);
+
 /* The norms before and after a residual block, with its gate and residual
  * scale, in one pass (all [rows, cols], one dtype, fp32 math):
  *   h_out = residual_scale * residual + gate * rms(x) * post_weight

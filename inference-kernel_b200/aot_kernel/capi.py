@@ -66,6 +66,7 @@ SIGNATURES: dict[str, list] = {
     "aotk_mxfp4_quantize": [_ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr],
     "aotk_mxfp4_dequantize": [_ptr, _ptr, _ptr, _i64, _i64, _int, _ptr],
     "aotk_mxfp4_gemm": [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _int, _ptr],
+    "aotk_mxfp4_gemm_path": [_i64, _i64, _i64, _int, ctypes.POINTER(ctypes.c_int)],
     "aotk_sandwich_rmsnorm": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64,
                               ctypes.c_double, _i64, _i64, ctypes.c_double, _int, _ptr],
 }
@@ -317,6 +318,16 @@ def mxfp4_dequantize(out, codes, scales, rows, cols, dtype, stream=None) -> None
 def mxfp4_gemm(c, a, a_scales, b, b_scales, M, N, K, out_dtype, stream=None) -> None:
     _call("aotk_mxfp4_gemm", _p(c), _p(a), _p(a_scales), _p(b), _p(b_scales), M, N, K, out_dtype,
           _stream(stream))
+
+
+MXFP4_PATHS = {0: "split", 1: "pair_256", 2: "pair_128", 3: "one_128", 4: "one_64"}
+
+
+def mxfp4_gemm_path(M, N, K, sm_count) -> str:
+    """The kernel aotk_mxfp4_gemm runs for a problem (host arithmetic)."""
+    p = ctypes.c_int(-1)
+    _call("aotk_mxfp4_gemm_path", M, N, K, sm_count, ctypes.byref(p))
+    return MXFP4_PATHS[p.value]
 
 
 def sandwich_rmsnorm(out, h_out, x, residual, post_weight, pre_weight, gate, gate_rows, gate_cols,

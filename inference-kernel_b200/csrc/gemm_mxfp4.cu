@@ -553,27 +553,6 @@ int launch_tiles(void* c, const void* a, const void* as, const void* b, const vo
   return check_launch("aotk_mxfp4_gemm");
 }
 
-template <typename T>
-int dispatch(void* c, const void* a, const void* as, const void* b, const void* bs, int M, int N,
-             int K, cudaStream_t s, const DeviceInfo& info) {
-  // Rounds of tiles on the SMs, times what a round takes against one of 256-column
-  // pairs (per 256 of K at full load 0.40 us; 0.29, 0.31 and 0.23 for the others).
-  auto cost = [&](int cg, int bn, double round) {
-    const int64_t workers = info.sm_count / cg;
-    return round * static_cast<double>((tile_count(cg, bn, M, N) + workers - 1) / workers);
-  };
-  const double pair256 = cost(2, 256, 1.0), pair128 = cost(2, 128, 0.7);
-  const double one128 = cost(1, 128, 0.77), one64 = cost(1, 64, 0.58);
-  const double pairs = pair256 < pair128 ? pair256 : pair128;
-  const double ones = one128 < one64 ? one128 : one64;
-  if (pairs <= ones) {
-    if (pair256 <= pair128) return launch_tiles<T, 2, 256, 6, 1>(c, a, as, b, bs, M, N, K, s, info);
-    return launch_tiles<T, 2, 128, 8, 1>(c, a, as, b, bs, M, N, K, s, info);
-  }
-  if (one128 <= one64) return launch_tiles<T, 1, 128, 6, 1>(c, a, as, b, bs, M, N, K, s, info);
-  return launch_tiles<T, 1, 64, 4, 2>(c, a, as, b, bs, M, N, K, s, info);
-}
-
 // Whether M <= 128 rows go to the kernel that splits K and streams the weight at two
 // CTAs per SM (gemm_mxfp4_skinny.cu) or to one-CTA tiles.  The former's exchange of
 // partial sums grows with M, the latter go through K one block after the other; up
@@ -581,12 +560,12 @@ int dispatch(void* c, const void* a, const void* as, const void* b, const void* 
 // weight from HBM (split / 64-column tiles / 128-column tiles measured): 128 rows,
 // N x K = 6144 x 4096 12.3 / 6.6 / 7.6, 4096 x 14336 13.2 / 13.3 / 16.7, 28672 x 4096
 // 17.2 / 19.0 / 15.8, 1024 x 8192 8.2 / 9.0 / 11.1; 64 rows, 28672 x 4096 14.5 / 18 / 15.
-bool prefer_split(int M, int N, int K, const DeviceInfo& info) {
+bool prefer_split(int M, int N, int K, int sm_count) {
   if (M <= 32) return true;
   const double weight_kb = static_cast<double>(N) * K * (17.0 / 32) / 1024;
   const int kblocks = (K - 1) / kBK + 1;
   auto tiles = [&](int bn, double per_block) {
-    const int64_t rounds = (tile_count(1, bn, M, N) + info.sm_count - 1) / info.sm_count;
+    const int64_t rounds = (tile_count(1, bn, M, N) + sm_count - 1) / sm_count;
     const double loop = per_block * kblocks * static_cast<double>(rounds);
     const double stream = weight_kb / 5100;
     return 3.8 + (loop > stream ? loop : stream);
@@ -594,6 +573,54 @@ bool prefer_split(int M, int N, int K, const DeviceInfo& info) {
   const double t64 = tiles(64, 0.167), t128 = tiles(128, 0.241);
   const double split = 2.5 + 0.039 * M + weight_kb / 4900;
   return split <= t64 && split <= t128;
+}
+
+// The kernel for a problem (AOTK_MXFP4_*).
+int path_of(int M, int N, int K, int sm_count) {
+  if (M <= kSkinnyMaxM && prefer_split(M, N, K, sm_count)) return AOTK_MXFP4_SPLIT;
+  // Rounds of tiles on the SMs, times what a round takes against one of 256-column
+  // pairs (per 256 of K at full load 0.40 us; 0.29, 0.31 and 0.23 for the others).
+  auto cost = [&](int cg, int bn, double round) {
+    const int64_t workers = sm_count / cg;
+    return round * static_cast<double>((tile_count(cg, bn, M, N) + workers - 1) / workers);
+  };
+  const double pair256 = cost(2, 256, 1.0), pair128 = cost(2, 128, 0.7);
+  const double one128 = cost(1, 128, 0.77), one64 = cost(1, 64, 0.58);
+  const double pairs = pair256 < pair128 ? pair256 : pair128;
+  const double ones = one128 < one64 ? one128 : one64;
+  if (pairs <= ones) return pair256 <= pair128 ? AOTK_MXFP4_PAIR_256 : AOTK_MXFP4_PAIR_128;
+  return one128 <= one64 ? AOTK_MXFP4_ONE_128 : AOTK_MXFP4_ONE_64;
+}
+
+template <typename T>
+int dispatch(int path, void* c, const void* a, const void* as, const void* b, const void* bs, int M,
+             int N, int K, cudaStream_t s, const DeviceInfo& info) {
+  switch (path) {
+    case AOTK_MXFP4_PAIR_256:
+      return launch_tiles<T, 2, 256, 6, 1>(c, a, as, b, bs, M, N, K, s, info);
+    case AOTK_MXFP4_PAIR_128:
+      return launch_tiles<T, 2, 128, 8, 1>(c, a, as, b, bs, M, N, K, s, info);
+    case AOTK_MXFP4_ONE_128:
+      return launch_tiles<T, 1, 128, 6, 1>(c, a, as, b, bs, M, N, K, s, info);
+    default: return launch_tiles<T, 1, 64, 4, 2>(c, a, as, b, bs, M, N, K, s, info);
+  }
+}
+
+// Arguments that do not depend on memory or a device.
+int check_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 0) return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: negative size", who);
+  if (K % 32 != 0)
+    return fail(AOTK_ERR_UNSUPPORTED, "%s: K = %lld is not a multiple of the block size 32", who,
+                (long long)K);
+  return AOTK_OK;
+}
+
+int check_limits(const char* who, int64_t M, int64_t N, int64_t K) {
+  if (M > 0x7fffff00LL || N > 0x7fffff00LL)
+    return fail(AOTK_ERR_UNSUPPORTED, "%s: extents above 2^31 - 256", who);
+  if (K > kMaxK)
+    return fail(AOTK_ERR_UNSUPPORTED, "%s: K = %lld is above 2^28", who, (long long)K);
+  return AOTK_OK;
 }
 
 }  // namespace
@@ -618,19 +645,13 @@ extern "C" int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, con
                                int out_dtype, void* stream) {
   using namespace aotk;
   const char* who = "aotk_mxfp4_gemm";
-  if (M < 0 || N < 0 || K < 0) return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: negative size", who);
+  if (int st = check_sizes(who, M, N, K)) return st;
   if (!valid_dtype(out_dtype))
     return fail(AOTK_ERR_UNSUPPORTED, "%s: unsupported output dtype %d", who, out_dtype);
-  if (K % 32 != 0)
-    return fail(AOTK_ERR_UNSUPPORTED, "%s: K = %lld is not a multiple of the block size 32", who,
-                (long long)K);
   if (M == 0 || N == 0) return AOTK_OK;
   if (!c || (K > 0 && (!a || !a_scales || !b || !b_scales)))
     return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  if (M > 0x7fffff00LL || N > 0x7fffff00LL)
-    return fail(AOTK_ERR_UNSUPPORTED, "%s: extents above 2^31 - 256", who);
-  if (K > kMaxK)
-    return fail(AOTK_ERR_UNSUPPORTED, "%s: K = %lld is above 2^28", who, (long long)K);
+  if (int st = check_limits(who, M, N, K)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (K == 0) {  // an empty sum
     const size_t bytes = static_cast<size_t>(M) * static_cast<size_t>(N) * elem_size(out_dtype);
@@ -643,11 +664,23 @@ extern "C" int aotk_mxfp4_gemm(void* c, const void* a, const void* a_scales, con
   if (int st = current_device_info(&info)) return st;
   if (int st = require_sm100(info)) return st;
   const int m = (int)M, n = (int)N, k = (int)K;
-  if (M <= kSkinnyMaxM && prefer_split(m, n, k, info))
+  const int path = path_of(m, n, k, info.sm_count);
+  if (path == AOTK_MXFP4_SPLIT)
     return gemm_mxfp4_skinny(c, a, a_scales, b, b_scales, m, n, k, out_dtype, stream, info);
   switch (out_dtype) {
-    case AOTK_FLOAT32: return dispatch<float>(c, a, a_scales, b, b_scales, m, n, k, s, info);
-    case AOTK_FLOAT16: return dispatch<__half>(c, a, a_scales, b, b_scales, m, n, k, s, info);
-    default: return dispatch<__nv_bfloat16>(c, a, a_scales, b, b_scales, m, n, k, s, info);
+    case AOTK_FLOAT32: return dispatch<float>(path, c, a, a_scales, b, b_scales, m, n, k, s, info);
+    case AOTK_FLOAT16: return dispatch<__half>(path, c, a, a_scales, b, b_scales, m, n, k, s, info);
+    default: return dispatch<__nv_bfloat16>(path, c, a, a_scales, b, b_scales, m, n, k, s, info);
   }
+}
+
+extern "C" int aotk_mxfp4_gemm_path(int64_t M, int64_t N, int64_t K, int sm_count, int* path) {
+  using namespace aotk;
+  const char* who = "aotk_mxfp4_gemm_path";
+  if (int st = check_sizes(who, M, N, K)) return st;
+  if (!path || M == 0 || N == 0 || K == 0 || sm_count < 2)
+    return fail(AOTK_ERR_INVALID_ARGUMENT, "%s: bad arguments", who);
+  if (int st = check_limits(who, M, N, K)) return st;
+  *path = path_of((int)M, (int)N, (int)K, sm_count);
+  return AOTK_OK;
 }
