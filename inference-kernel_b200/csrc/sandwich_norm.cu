@@ -9,12 +9,12 @@
 // HBM: the row lives in registers from its one read to its two writes, and the
 // two sums meet through warp shuffles and shared memory.  Three kernels:
 //   * sandwich_kernel: TPR threads per row hold it in registers, everything
-//     requested before the first sum: few rows, and rows of any length whose
-//     starts are not multiples of 16 bytes;
-//   * sandwich_ring_kernel: many rows of 1 to 48 KB (32 KB where they do not start on
-//     16 bytes), streamed through shared memory;
-//   * sandwich_long_kernel: rows that fit neither, or tensors that do not start
-//     on 16 bytes: the row is read three times.
+//     requested before the first sum: rows below 1 KB, few rows (less than 1 MB in
+//     all), and rows of up to 64 KB that are too long for the next;
+//   * sandwich_ring_kernel: 1 MB or more of rows of 1 to 48 KB (32 KB where they do not
+//     start on 16 bytes), streamed through shared memory;
+//   * sandwich_long_kernel: rows above 64 KB, or tensors that do not start on 16
+//     bytes: the row is read three times.
 //
 // Squares of bf16's and fp32's largest numbers (from about 1.8e19 on) and, with a
 // small eps, of their smallest leave fp32's range, where rms(v) itself is of order 1.
@@ -160,10 +160,12 @@ __device__ __forceinline__ void row_out_of_range(const Args<T>& a, int64_t row, 
 
 // The same out of line, for rows of a warp or less, of which there may be many at a time:
 // inlined it costs their kernels registers, and with them blocks per SM (16384 x 256 bf16
-// 7.7 us; inline 9.9).
+// 7.3 us; inline 9.9).
 template <typename T, int TPR>
-__device__ __noinline__ void row_out_of_range_call(const Args<T>& a, int64_t row, int t, int group) {
-  row_out_of_range<T, TPR>(a, row, t, group, nullptr);
+__device__ __noinline__ void row_out_of_range_call(const Args<T>& a) {
+  const int group = threadIdx.x / TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / TPR) + group;
+  row_out_of_range<T, TPR>(a, row, threadIdx.x % TPR, group, nullptr);
 }
 
 // Elements [pos + lo, pos + hi) of `base` in their places of a vector, one by one.
@@ -276,7 +278,7 @@ struct ShiftedWeight {
 constexpr int threads_for(int tpr) { return tpr > 256 ? tpr : 256; }
 
 // Blocks per SM that rows of a warp or less are compiled for, one of which the registers
-// of the call behind them would cost (65536 x 128 bf16 13.2 us; 16.9 with three blocks).
+// of the call behind them would cost (65536 x 128 bf16 13.1 us; 16.9 with three blocks).
 // Unaligned 16-bit rows of two vectors keep theirs, and lose if held to it (30000 x 99 fp16
 // 11.3 -> 12.0).
 template <typename T, bool kShift, int VPT, int TPR>
@@ -300,9 +302,10 @@ __global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, T
   constexpr int RPB = kThreads / TPR;
   // With 1024 threads the registers hold the row, but not its weights too.
   constexpr bool kEarly = TPR < 1024;
-  // Nor do the 64 that leave room for four blocks per SM: there the second weight comes
-  // after the first sum (65536 x 128 bf16 13.1 us; 16.6 with spills).
-  constexpr bool kPreLate = TPR <= 32 && std::is_same_v<T, __nv_bfloat16> && !kShift && VPT == 2;
+  // Nor do those that leave room for three to five blocks per SM: there the second weight
+  // of 16-bit rows comes before the second sum (16384 x 256 bf16 7.3 us, 65536 x 128 13.1;
+  // 9.9 and 16.6 with spills).
+  constexpr bool kPreLate = TPR <= 32 && sizeof(T) == 2;
   __shared__ float buf[2][kThreads / 32];
   const int t = threadIdx.x % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
@@ -421,12 +424,7 @@ __global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, T
   const float sum = row_sum<TPR>(ss.x + ss.y, buf[0]);
   const float mean = sum / static_cast<float>(a.cols) + a.eps;
   const float inv = rsqrtf(mean);
-
-  if constexpr (kPreLate) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (used(i)) load_pre(i);
-  }
+  bool again = live && out_of_range(mean);
 
   ss = make_float2(0.f, 0.f);
   const float scale = inv * g_row;
@@ -453,9 +451,15 @@ __global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, T
       write(a.h_out, column(i), h[i]);
     }
   }
+  if constexpr (kPreLate) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (used(i)) load_pre(i);
+  }
   const float sum_h = row_sum<TPR>(ss.x + ss.y, buf[1]);
   const float mean_h = sum_h / static_cast<float>(a.cols) + a.eps;
   const float inv_h = rsqrtf(mean_h);
+  again |= live && out_of_range(mean_h);
   const float2 inv_h2 = make_float2(inv_h, inv_h);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -469,10 +473,10 @@ __global__ void __launch_bounds__(threads_for(TPR), blocks_for<T, kShift, VPT, T
     }
   }
   // The row's threads have the same sums.
-  if (live && (out_of_range(mean) | out_of_range(mean_h))) {
+  if (again) {
     const int group = threadIdx.x / TPR;
     if constexpr (TPR <= 32)
-      row_out_of_range_call<T, TPR>(a, row, t, group);
+      row_out_of_range_call<T, TPR>(a);
     else
       row_out_of_range<T, TPR>(a, row, t, group, buf[0] + group * (TPR / 32));
   }
@@ -969,7 +973,9 @@ int launch_ring(const Args<T>& a, cudaStream_t s, const DeviceInfo& info) {
 // The smallest group that holds a row in few vectors per thread: four of fp32, three
 // of 16-bit types, whose four would not fit the registers beside their weights
 // (20000 x 1001 bf16 45.0 -> 33.9 us, 8192 x 4096 48.0 -> 45.1; fp32 8192 x 4096 is
-// 89.5 with four and 95.2 with two).
+// 89.5 with four and 95.2 with two).  Three of unaligned fp16 rows spill 36 to 44 bytes
+// all the same, and run as fast as those of bf16, which do not (20000 x 1001 30.6 us;
+// 32.6).
 template <typename T, bool kShift, int TPR>
 int dispatch_group(const Args<T>& a, int n, cudaStream_t s, const DeviceInfo& info) {
   if (n <= 2 * TPR) return launch_ring<T, kShift, 2, TPR>(a, s, info);
