@@ -23,10 +23,12 @@
 //     do not start on 16 bytes, the memory of one or two stages turns the rows for
 //     stores along them.
 // What bounds it: tiles of one CTA by operand traffic out of L2, about 16.5 TB/s
-// over the chip (128 x 256 tiles: 51 KB per 256 of K, 0.455 us where the MMAs take
-// 0.27); pairs of CTAs move 35 KB for the same work and end at the power cap.  64
-// columns are bound by the work per stage of the issuing warps, hence SUB = 2 there
-// (128 x 6144 x 4096 7.1 -> 6.6 us, 128 x 4096 x 14336 15.2 -> 13.3).  Sending the
+// over the chip.  128 x 256 tiles moved 51 KB per 256 of K, 0.455 us where the MMAs
+// take 0.27; the pairs of CTAs that took their place move 35 KB for the same work and
+// end at the power cap.  Of the one-CTA tiles left, for grids that do not fill the
+// chip with pairs, 128 x 64 ones are bound by the work per stage of the issuing
+// warps, hence SUB = 2 there (128 x 6144 x 4096 7.1 -> 6.6 us, 128 x 4096 x 14336
+// 15.2 -> 13.3).  Sending the
 // scales a stage ahead of their MMAs, or between them, gained nothing or lost.
 // K is padded by zeros (TMA fill); MMAs stop at the last 64 elements that exist.
 // Rows beyond M or N may multiply stale or foreign scales, and are not stored.
